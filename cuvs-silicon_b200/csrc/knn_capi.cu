@@ -41,6 +41,7 @@
 
 #include "cuvs_b200.h"
 #include "knn_internal.h"
+#include "knn_store.h"
 
 using knn::Plan;
 
@@ -1684,6 +1685,12 @@ uint64_t knn_dispatch_count(void) { return g_dispatch.load(); }
 void knn_reset_dispatch_count(void) { g_dispatch.store(0); }
 
 }  // extern "C"
+
+// The row store's entry points (knn_store_capi.cu) report and count here too.
+namespace knn {
+int store_fail(int status, const char* text) { return fail(status, "%s", text); }
+void store_count_launches(int n) { g_dispatch.fetch_add(static_cast<uint64_t>(n)); }
+}  // namespace knn
 
 // ---------------------------------------------------------------------------
 // Search without allocation (knn_index_search_noalloc).

@@ -1,0 +1,727 @@
+// knn_pages.cu -- pages of rows: growing, copying, forking, compacting and
+// freeing them.
+//
+// A store is a table of page numbers for every sequence, the sequences'
+// lengths in rows, a count of references for every page, and up to
+// KNN_PAGES_MAX_POOLS pools [pages][page_rows][row bytes] that share the page
+// numbers.  Row j of sequence s is row j % page_rows of page
+// table[s][j / page_rows].  A page with no references is free; there is no
+// list of free pages that could disagree with the counts.
+//
+// Fresh pages are always the lowest-numbered free ones, given out in the
+// order of the call's list, so that results never depend on the order in
+// which threads run.  A call that breaks a rule (an index out of range, a
+// target listed twice, too few free pages, ...) changes nothing: the kernel
+// that plans it records the error and clears status[1] ("applied"), and the
+// kernels that move data check that word first.
+//
+// What bounds them: planning is a latency (one CTA: a list of a few
+// sequences, a scan of the counts), moving rows is HBM bandwidth.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "knn_store.h"
+
+namespace knn {
+
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kMaxList = KNN_PAGES_MAX_LIST;
+constexpr int kMoveThreads = 256;
+constexpr int64_t kMoveChunk = 16384;  // bytes of a page that one CTA moves at a time
+constexpr int kShareChunk = 1024;      // table entries that one CTA shares at a time
+constexpr int kKeepChunk = 128;        // positions of a sequence that one CTA compacts
+
+// ------------------------------------------------------------ plan kernels
+struct PlanSmem {
+  unsigned long long part[kPlanWarps];
+  unsigned long long total;
+  int bad;
+};
+
+// Exclusive prefix sum over the block; *total gets the sum.
+__device__ unsigned long long block_exclusive(unsigned long long v, PlanSmem& sm,
+                                              unsigned long long* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  unsigned long long inc = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const unsigned long long o = __shfl_up_sync(0xffffffffu, inc, d);
+    if (lane >= d) inc += o;
+  }
+  __syncthreads();  // the last call's readers are done with part and total
+  if (lane == 31) sm.part[warp] = inc;
+  __syncthreads();
+  if (warp == 0) {
+    unsigned long long w = sm.part[lane], s = w;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const unsigned long long o = __shfl_up_sync(0xffffffffu, s, d);
+      if (lane >= d) s += o;
+    }
+    sm.part[lane] = s - w;
+    if (lane == 31) sm.total = s;
+  }
+  __syncthreads();
+  *total = sm.total;
+  return sm.part[warp] + inc - v;
+}
+
+// Sets a bit of a shared bitmap; false if it was set already.
+__device__ __forceinline__ bool mark(uint32_t* bits, int64_t i) {
+  const uint32_t m = 1u << (i & 31);
+  return (atomicOr(&bits[i >> 5], m) & m) == 0;
+}
+
+__device__ __forceinline__ void raise(PlanSmem& sm, int code) { atomicCAS(&sm.bad, 0, code); }
+
+// Ends a plan: records an error and whether the call goes on.  All threads.
+__device__ bool plan_goes_on(const knn_pages& p, PlanSmem& sm) {
+  __syncthreads();
+  const int bad = sm.bad;
+  if (threadIdx.x == 0) {
+    if (bad) atomicCAS(&p.status[kStatusError], 0, bad);
+    p.status[kStatusApplied] = bad == 0;
+  }
+  return bad == 0;
+}
+
+// Gives out the `need` lowest-numbered free pages: give(rank, page) for ranks
+// 0 .. need - 1 in order of the page numbers.  Returns how many there were.
+// The block reads the counts in tiles of 16 a thread, four 16-byte loads
+// that are each coalesced; the four runs of a tile are ranked by one prefix
+// sum over four 16-bit fields (a run counts at most 4096).
+template <class Give>
+__device__ int take_free(const knn_pages& p, int need, PlanSmem& sm, Give give) {
+  constexpr int kRun = 4 * kPlanThreads;
+  int given = 0;
+  for (int64_t base = 0; base < p.pages && given < need; base += 4 * kRun) {
+    int4 r[4];
+    unsigned long long count = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t i = base + j * kRun + 4 * threadIdx.x;
+      if (i + 4 <= p.pages && (reinterpret_cast<uintptr_t>(p.refs) & 15) == 0) {
+        r[j] = *reinterpret_cast<const int4*>(p.refs + i);
+      } else {
+        r[j].x = i < p.pages ? p.refs[i] : 1;
+        r[j].y = i + 1 < p.pages ? p.refs[i + 1] : 1;
+        r[j].z = i + 2 < p.pages ? p.refs[i + 2] : 1;
+        r[j].w = i + 3 < p.pages ? p.refs[i + 3] : 1;
+      }
+      const int c = (r[j].x == 0) + (r[j].y == 0) + (r[j].z == 0) + (r[j].w == 0);
+      count |= static_cast<unsigned long long>(c) << (16 * j);
+    }
+    unsigned long long total;
+    const unsigned long long before = block_exclusive(count, sm, &total);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t i = base + j * kRun + 4 * threadIdx.x;
+      int rank = given + static_cast<int>((before >> (16 * j)) & 0xffff);
+      if (r[j].x == 0 && rank < need) give(rank, static_cast<int32_t>(i));
+      rank += r[j].x == 0;
+      if (r[j].y == 0 && rank < need) give(rank, static_cast<int32_t>(i + 1));
+      rank += r[j].y == 0;
+      if (r[j].z == 0 && rank < need) give(rank, static_cast<int32_t>(i + 2));
+      rank += r[j].z == 0;
+      if (r[j].w == 0 && rank < need) give(rank, static_cast<int32_t>(i + 3));
+      given += static_cast<int>((total >> (16 * j)) & 0xffff);
+    }
+  }
+  return given < need ? given : need;
+}
+
+// Index of the run that rank falls in: the last i with first[i] <= rank.
+__device__ __forceinline__ int run_of(const int32_t* first, int n, int rank) {
+  int low = 0, high = n - 1;
+  while (low < high) {
+    const int mid = (low + high + 1) >> 1;
+    if (first[mid] <= rank) low = mid;
+    else high = mid - 1;
+  }
+  return low;
+}
+
+__device__ __forceinline__ int64_t pages_for(int64_t rows, int page_rows) {
+  return (rows + page_rows - 1) / page_rows;
+}
+
+// grow: counts[i] more rows for sequence seqs[i].
+__global__ void __launch_bounds__(kPlanThreads) grow_kernel(knn_pages p, const int32_t* seqs,
+                                                            const int32_t* counts, int n,
+                                                            int64_t wanted) {
+  extern __shared__ uint32_t dyn[];
+  __shared__ PlanSmem sm;
+  int32_t* first = reinterpret_cast<int32_t*>(dyn);  // [n + 1] pages before entry i
+  uint32_t* seen = dyn + n + 1;                      // bitmap of the sequences
+  const int64_t words = (p.sequences + 31) / 32;
+  if (threadIdx.x == 0) sm.bad = 0;
+  for (int64_t i = threadIdx.x; i < words; i += kPlanThreads) seen[i] = 0;
+  wait_for_stream();
+  __syncthreads();
+  constexpr int kPer = kMaxList / kPlanThreads;
+  unsigned long long fresh[kPer], mine = 0, rows_sum = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int i = threadIdx.x * kPer + j;
+    fresh[j] = 0;
+    if (i >= n) continue;
+    const int64_t s = seqs[i], c = counts[i];
+    if (s < 0 || s >= p.sequences) raise(sm, KNN_PAGES_OUT_OF_RANGE);
+    else if (c < 0) raise(sm, KNN_PAGES_BAD_COUNT);
+    else if (!mark(seen, s)) raise(sm, KNN_PAGES_LISTED_TWICE);
+    else {
+      const int64_t length = p.rows[s];
+      const int64_t after = pages_for(length + c, p.page_rows);
+      if (length < 0 || after > p.columns || length + c > 0x7fffffff) raise(sm, KNN_PAGES_TOO_LONG);
+      else fresh[j] = after - pages_for(length, p.page_rows);
+      rows_sum += c;
+    }
+    mine += fresh[j];
+  }
+  unsigned long long need = 0, rows_total = 0;
+  unsigned long long before = block_exclusive(mine, sm, &need);
+  block_exclusive(rows_sum, sm, &rows_total);
+  if (wanted >= 0 && rows_total != static_cast<unsigned long long>(wanted))
+    raise(sm, KNN_PAGES_BAD_COUNT);
+  if (need > static_cast<unsigned long long>(p.pages)) raise(sm, KNN_PAGES_NONE_FREE);
+  __syncthreads();
+  if (sm.bad == 0) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int i = threadIdx.x * kPer + j;
+      if (i < n) first[i] = static_cast<int32_t>(before);
+      before += fresh[j];
+    }
+    __syncthreads();
+    auto entry = [&](int rank) -> int32_t* {
+      const int i = run_of(first, n, rank);
+      const int64_t s = seqs[i];
+      return p.table + s * p.columns + pages_for(p.rows[s], p.page_rows) + (rank - first[i]);
+    };
+    const int want = static_cast<int>(need);
+    const int got = take_free(p, want, sm, [&](int rank, int32_t page) {
+      *entry(rank) = page;
+      p.refs[page] = 1;
+    });
+    __syncthreads();
+    if (got < want) {  // too few: give them back
+      for (int rank = threadIdx.x; rank < got; rank += kPlanThreads) {
+        int32_t* e = entry(rank);
+        p.refs[*e] = 0;
+        *e = -1;
+      }
+      raise(sm, KNN_PAGES_NONE_FREE);
+    }
+  }
+  if (!plan_goes_on(p, sm)) return;
+  for (int i = threadIdx.x; i < n; i += kPlanThreads) p.rows[seqs[i]] += counts[i];
+}
+
+// ------------------------------------------------------------------- free
+// One CTA a listed sequence.  Every CTA looks the whole list over (a few KB
+// out of L2), so that a bad index stops all of them; a sequence that is
+// listed again is freed by its first mention alone.
+__global__ void __launch_bounds__(kMoveThreads) free_kernel(knn_pages p, const int32_t* seqs,
+                                                            int n) {
+  wait_for_stream();
+  const int i = blockIdx.x;
+  const int32_t s = seqs[i];
+  bool bad = false, again = false;
+  for (int j = threadIdx.x; j < n; j += kMoveThreads) {
+    const int32_t o = seqs[j];
+    bad |= o < 0 || o >= p.sequences;
+    again |= j < i && o == s;
+  }
+  bad = __syncthreads_or(bad);
+  again = __syncthreads_or(again);
+  if (i == 0 && threadIdx.x == 0) {
+    if (bad) atomicCAS(&p.status[kStatusError], 0, KNN_PAGES_OUT_OF_RANGE);
+    p.status[kStatusApplied] = !bad;
+  }
+  if (bad || again) return;
+  int64_t used = pages_for(p.rows[s], p.page_rows);
+  if (used > p.columns) used = p.columns;
+  for (int64_t c = threadIdx.x; c < used; c += kMoveThreads) {
+    int32_t* e = p.table + s * p.columns + c;
+    const int32_t page = *e;
+    if (page >= 0 && page < p.pages) atomicSub(&p.refs[page], 1);
+    *e = -1;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) p.rows[s] = 0;
+}
+
+// ------------------------------------------------------------------- moves
+// Copies `bytes` bytes with all threads of the block, 16 at a time where
+// both ends allow it.
+__device__ __forceinline__ void block_copy(uint8_t* to, const uint8_t* from, int64_t bytes) {
+  if (((reinterpret_cast<uintptr_t>(to) | reinterpret_cast<uintptr_t>(from)) & 15) == 0) {
+    const int64_t n = bytes >> 4;
+    const uint4* f = reinterpret_cast<const uint4*>(from);
+    uint4* t = reinterpret_cast<uint4*>(to);
+    int64_t i = threadIdx.x;
+    for (; i + 3 * kMoveThreads < n; i += 4 * kMoveThreads) {
+      uint4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = __ldcs(f + i + j * kMoveThreads);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) __stcs(t + i + j * kMoveThreads, v[j]);
+    }
+    for (; i < n; i += kMoveThreads) __stcs(t + i, __ldcs(f + i));
+    for (int64_t b = (n << 4) + threadIdx.x; b < bytes; b += kMoveThreads) to[b] = from[b];
+  } else {
+    for (int64_t b = threadIdx.x; b < bytes; b += kMoveThreads) to[b] = from[b];
+  }
+}
+
+// copy, plan: every index in range, no target twice, no target a source.
+__global__ void __launch_bounds__(kPlanThreads) copy_plan_kernel(knn_pages p,
+                                                                 const int32_t* sources,
+                                                                 const int32_t* targets,
+                                                                 int64_t n) {
+  extern __shared__ uint32_t dyn[];
+  __shared__ PlanSmem sm;
+  const int64_t words = (p.pages + 31) / 32;
+  if (threadIdx.x == 0) sm.bad = 0;
+  for (int64_t i = threadIdx.x; i < words; i += kPlanThreads) dyn[i] = 0;
+  wait_for_stream();
+  __syncthreads();
+  for (int64_t i = threadIdx.x; i < n; i += kPlanThreads) {
+    const int32_t t = targets[i];
+    if (t < 0 || t >= p.pages) raise(sm, KNN_PAGES_OUT_OF_RANGE);
+    else if (!mark(dyn, t)) raise(sm, KNN_PAGES_LISTED_TWICE);
+  }
+  __syncthreads();
+  for (int64_t i = threadIdx.x; i < n; i += kPlanThreads) {
+    const int32_t s = sources[i];
+    if (s < 0 || s >= p.pages) raise(sm, KNN_PAGES_OUT_OF_RANGE);
+    else if ((dyn[s >> 5] >> (s & 31)) & 1) raise(sm, KNN_PAGES_LISTED_TWICE);
+  }
+  plan_goes_on(p, sm);
+}
+
+__global__ void __launch_bounds__(kMoveThreads) copy_kernel(knn_pages p, const int32_t* sources,
+                                                            const int32_t* targets, int64_t n,
+                                                            int64_t chunks) {
+  wait_for_stream();
+  if (!p.status[kStatusApplied]) return;
+  for (int64_t item = blockIdx.x; item < n * chunks; item += gridDim.x) {
+    const int64_t i = item / chunks;
+    int64_t chunk = item - i * chunks;
+    for (int k = 0; k < p.n_pools; ++k) {
+      const int64_t bytes = p.row_bytes[k] * p.page_rows;
+      const int64_t parts = (bytes + kMoveChunk - 1) / kMoveChunk;
+      if (chunk < parts) {
+        uint8_t* pool = static_cast<uint8_t*>(p.pools[k]);
+        const int64_t off = chunk * kMoveChunk;
+        const int64_t left = bytes - off;
+        block_copy(pool + targets[i] * bytes + off, pool + sources[i] * bytes + off,
+                   left < kMoveChunk ? left : kMoveChunk);
+        break;
+      }
+      chunk -= parts;
+    }
+  }
+}
+
+// -------------------------------------------------------------------- fork
+// fork, plan: the children's lengths, and a fresh page for each child whose
+// parent's last page is not full.
+__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(knn_pages p,
+                                                                 const int32_t* parents,
+                                                                 const int32_t* children, int n) {
+  extern __shared__ uint32_t dyn[];
+  __shared__ PlanSmem sm;
+  int32_t* who = reinterpret_cast<int32_t*>(dyn);  // [n] the children that need a page
+  int32_t* length = who + n;                       // [n] their parents' lengths
+  uint32_t* seen = dyn + 2 * n;
+  const int64_t words = (p.sequences + 31) / 32;
+  if (threadIdx.x == 0) sm.bad = 0;
+  for (int64_t i = threadIdx.x; i < words; i += kPlanThreads) seen[i] = 0;
+  wait_for_stream();
+  __syncthreads();
+  constexpr int kPer = kMaxList / kPlanThreads;
+  unsigned long long mine = 0;
+  bool part[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int i = threadIdx.x * kPer + j;
+    part[j] = false;
+    if (i >= n) continue;
+    const int64_t s = parents[i], c = children[i];
+    if (s < 0 || s >= p.sequences || c < 0 || c >= p.sequences) raise(sm, KNN_PAGES_OUT_OF_RANGE);
+    else if (!mark(seen, c)) raise(sm, KNN_PAGES_LISTED_TWICE);
+    else if (p.rows[c] != 0) raise(sm, KNN_PAGES_NOT_EMPTY);
+    else {
+      const int32_t rows = p.rows[s];
+      if (rows < 0 || pages_for(rows, p.page_rows) > p.columns) raise(sm, KNN_PAGES_TOO_LONG);
+      length[i] = rows;
+      part[j] = rows % p.page_rows != 0;
+    }
+    mine += part[j];
+  }
+  unsigned long long need = 0;
+  int before = static_cast<int>(block_exclusive(mine, sm, &need));
+#pragma unroll
+  for (int j = 0; j < kPer; ++j)
+    if (part[j]) who[before++] = threadIdx.x * kPer + j;
+  __syncthreads();
+  if (sm.bad == 0 && need > 0) {
+    auto entry = [&](int rank) {
+      const int i = who[rank];
+      return p.table + children[i] * p.columns + length[i] / p.page_rows;
+    };
+    const int want = static_cast<int>(need);
+    const int got = take_free(p, want, sm, [&](int rank, int32_t page) {
+      *entry(rank) = page;
+      p.refs[page] = 1;
+    });
+    __syncthreads();
+    if (got < want) {
+      for (int rank = threadIdx.x; rank < got; rank += kPlanThreads) {
+        int32_t* e = entry(rank);
+        p.refs[*e] = 0;
+        *e = -1;
+      }
+      raise(sm, KNN_PAGES_NONE_FREE);
+    }
+  }
+  if (!plan_goes_on(p, sm)) return;
+  for (int i = threadIdx.x; i < n; i += kPlanThreads) p.rows[children[i]] = length[i];
+}
+
+// fork, move: full pages are shared (table entry, one more reference), the
+// rows of a part-filled last page are copied.
+__global__ void __launch_bounds__(kMoveThreads) fork_kernel(knn_pages p, const int32_t* parents,
+                                                            const int32_t* children, int64_t n,
+                                                            int64_t shares, int64_t chunks) {
+  wait_for_stream();
+  if (!p.status[kStatusApplied]) return;
+  const int64_t per = shares + chunks;
+  for (int64_t item = blockIdx.x; item < n * per; item += gridDim.x) {
+    const int64_t i = item / per;
+    int64_t part = item - i * per;
+    const int64_t s = parents[i], c = children[i];
+    const int64_t length = p.rows[c];
+    const int64_t full = length / p.page_rows;
+    const int32_t* theirs = p.table + s * p.columns;
+    int32_t* ours = p.table + c * p.columns;
+    if (part < shares) {
+      int64_t end = (part + 1) * kShareChunk;
+      if (end > full) end = full;
+      for (int64_t col = part * kShareChunk + threadIdx.x; col < end; col += kMoveThreads) {
+        const int32_t page = theirs[col];
+        ours[col] = page;
+        if (page >= 0 && page < p.pages) atomicAdd(&p.refs[page], 1);
+      }
+      continue;
+    }
+    part -= shares;
+    const int64_t tail = length - full * p.page_rows;
+    if (tail == 0) continue;
+    const int32_t from = theirs[full], to = ours[full];
+    if (from < 0 || from >= p.pages) continue;
+    for (int k = 0; k < p.n_pools; ++k) {
+      const int64_t page_bytes = p.row_bytes[k] * p.page_rows;
+      const int64_t parts = (page_bytes + kMoveChunk - 1) / kMoveChunk;
+      if (part < parts) {
+        uint8_t* pool = static_cast<uint8_t*>(p.pools[k]);
+        const int64_t off = part * kMoveChunk;
+        const int64_t left = tail * p.row_bytes[k] - off;
+        if (left > 0)
+          block_copy(pool + to * page_bytes + off, pool + from * page_bytes + off,
+                     left < kMoveChunk ? left : kMoveChunk);
+        break;
+      }
+      part -= parts;
+    }
+  }
+}
+
+// ----------------------------------------------------------------- compact
+// Workspace: kept[n][chunks] rows kept in each chunk of kKeepChunk positions
+// (then, after the plan, those kept before it), total[n], fresh[n][columns].
+struct CompactWork {
+  int32_t* kept;
+  int32_t* total;
+  int32_t* fresh;
+  int64_t chunks;
+};
+
+__global__ void __launch_bounds__(kKeepChunk) compact_count_kernel(
+    knn_pages p, const int32_t* sources, const uint8_t* keep, int64_t keep_columns,
+    int64_t keep_stride, CompactWork w) {
+  wait_for_stream();
+  const int64_t i = blockIdx.x / w.chunks, chunk = blockIdx.x % w.chunks;
+  const int64_t s = sources[i];
+  const int64_t length = s >= 0 && s < p.sequences ? p.rows[s] : 0;
+  const int64_t at = chunk * kKeepChunk + threadIdx.x;
+  const bool kept = at < keep_columns && at < length && keep[i * keep_stride + at] != 0;
+  const int count = __syncthreads_count(kept);
+  if (threadIdx.x == 0) w.kept[i * w.chunks + chunk] = count;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(knn_pages p,
+                                                                    const int32_t* sources,
+                                                                    const int32_t* targets, int n,
+                                                                    int64_t keep_columns,
+                                                                    CompactWork w) {
+  extern __shared__ uint32_t dyn[];
+  __shared__ PlanSmem sm;
+  int32_t* first = reinterpret_cast<int32_t*>(dyn);  // [n]
+  uint32_t* seen = dyn + n;
+  const int64_t words = (p.sequences + 31) / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) sm.bad = 0;
+  for (int64_t i = threadIdx.x; i < words; i += kPlanThreads) seen[i] = 0;
+  wait_for_stream();
+  // rows kept before each chunk, a warp to a sequence
+  for (int64_t i = warp; i < n; i += kPlanWarps) {
+    int32_t* kept = w.kept + i * w.chunks;
+    int sum = 0;
+    for (int64_t base = 0; base < w.chunks; base += 32) {
+      const int64_t c = base + lane;
+      const int v = c < w.chunks ? kept[c] : 0;
+      int inc = v;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, inc, d);
+        if (lane >= d) inc += o;
+      }
+      if (c < w.chunks) kept[c] = sum + inc - v;
+      sum += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) w.total[i] = sum;
+  }
+  __syncthreads();
+  constexpr int kPer = kMaxList / kPlanThreads;
+  unsigned long long fresh[kPer], mine = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int i = threadIdx.x * kPer + j;
+    fresh[j] = 0;
+    if (i >= n) continue;
+    const int64_t s = sources[i], t = targets[i];
+    if (s < 0 || s >= p.sequences || t < 0 || t >= p.sequences) raise(sm, KNN_PAGES_OUT_OF_RANGE);
+    else if (!mark(seen, t)) raise(sm, KNN_PAGES_LISTED_TWICE);
+    else if (t != s && p.rows[t] != 0) raise(sm, KNN_PAGES_NOT_EMPTY);
+    else if (p.rows[s] > keep_columns) raise(sm, KNN_PAGES_BAD_COUNT);
+    else if (p.rows[s] < 0 || pages_for(p.rows[s], p.page_rows) > p.columns)
+      raise(sm, KNN_PAGES_TOO_LONG);
+    else fresh[j] = pages_for(w.total[i], p.page_rows);
+    mine += fresh[j];
+  }
+  unsigned long long need = 0;
+  unsigned long long before = block_exclusive(mine, sm, &need);
+  if (need > static_cast<unsigned long long>(p.pages)) raise(sm, KNN_PAGES_NONE_FREE);
+  __syncthreads();
+  if (sm.bad == 0) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int i = threadIdx.x * kPer + j;
+      if (i < n) first[i] = static_cast<int32_t>(before);
+      before += fresh[j];
+    }
+    __syncthreads();
+    auto entry = [&](int rank) {
+      const int i = run_of(first, n, rank);
+      return w.fresh + i * p.columns + (rank - first[i]);
+    };
+    const int want = static_cast<int>(need);
+    const int got = take_free(p, want, sm, [&](int rank, int32_t page) {
+      *entry(rank) = page;
+      p.refs[page] = 1;
+    });
+    __syncthreads();
+    if (got < want) {
+      for (int rank = threadIdx.x; rank < got; rank += kPlanThreads) p.refs[*entry(rank)] = 0;
+      raise(sm, KNN_PAGES_NONE_FREE);
+    }
+  }
+  plan_goes_on(p, sm);
+}
+
+// The kept rows of a chunk go to their places, piece by piece.
+template <class T>
+__device__ __forceinline__ void gather_rows(T* pool, const int64_t* from, const int64_t* to,
+                                            int kept, int64_t row_bytes) {
+  const uint32_t pieces = static_cast<uint32_t>(row_bytes / sizeof(T));
+  const uint32_t total = pieces * kept;
+  for (uint32_t i = threadIdx.x; i < total; i += kMoveThreads) {
+    const uint32_t r = i / pieces, c = i - r * pieces;
+    pool[to[r] * pieces + c] = pool[from[r] * pieces + c];
+  }
+}
+
+__global__ void __launch_bounds__(kMoveThreads) compact_kernel(knn_pages p, const int32_t* sources,
+                                                               const uint8_t* keep,
+                                                               int64_t keep_stride,
+                                                               CompactWork w) {
+  __shared__ int64_t from[kKeepChunk], to[kKeepChunk];
+  __shared__ int warp_kept[kKeepChunk / 32];
+  wait_for_stream();
+  if (!p.status[kStatusApplied]) return;
+  const int64_t i = blockIdx.x / w.chunks, chunk = blockIdx.x % w.chunks;
+  const int64_t s = sources[i];
+  const int64_t at = chunk * kKeepChunk + threadIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  bool kept = false;
+  unsigned ballot = 0;
+  if (threadIdx.x < kKeepChunk) {
+    kept = at < p.rows[s] && keep[i * keep_stride + at] != 0;
+    ballot = __ballot_sync(0xffffffffu, kept);
+    if (lane == 0) warp_kept[warp] = __popc(ballot);
+  }
+  __syncthreads();
+  int total = 0, before = 0;
+#pragma unroll
+  for (int j = 0; j < kKeepChunk / 32; ++j) {
+    if (j < warp) before += warp_kept[j];
+    total += warp_kept[j];
+  }
+  if (total == 0) return;
+  if (kept) {
+    const int slot = before + __popc(ballot & ((1u << lane) - 1));
+    const Places old = {p.table, p.columns, p.pages, p.page_rows};
+    const Places now = {w.fresh, p.columns, p.pages, p.page_rows};
+    const int64_t a = old.at(s, at);
+    from[slot] = a < 0 ? 0 : a;  // a table entry without a page: any row
+    to[slot] = now.at(i, w.kept[i * w.chunks + chunk] + slot);
+  }
+  __syncthreads();
+  for (int k = 0; k < p.n_pools; ++k) {
+    const int64_t bytes = p.row_bytes[k];
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(p.pools[k]) | static_cast<uintptr_t>(bytes);
+    if ((bits & 15) == 0) gather_rows(static_cast<uint4*>(p.pools[k]), from, to, total, bytes);
+    else if ((bits & 3) == 0) gather_rows(static_cast<uint32_t*>(p.pools[k]), from, to, total, bytes);
+    else gather_rows(static_cast<uint8_t*>(p.pools[k]), from, to, total, bytes);
+  }
+}
+
+// The targets' table rows and lengths; a target that is its own source lets
+// its old pages go.
+__global__ void __launch_bounds__(kMoveThreads) compact_commit_kernel(knn_pages p,
+                                                                      const int32_t* sources,
+                                                                      const int32_t* targets,
+                                                                      CompactWork w) {
+  wait_for_stream();
+  if (!p.status[kStatusApplied]) return;
+  const int64_t i = blockIdx.x;
+  const int64_t s = sources[i], t = targets[i];
+  const int64_t used = s == t ? pages_for(p.rows[t], p.page_rows) : 0;
+  const int64_t fresh = pages_for(w.total[i], p.page_rows);
+  int32_t* ours = p.table + t * p.columns;
+  for (int64_t c = threadIdx.x; c < (used > fresh ? used : fresh); c += kMoveThreads) {
+    if (c < used) {
+      const int32_t page = ours[c];
+      if (page >= 0 && page < p.pages) atomicSub(&p.refs[page], 1);
+    }
+    ours[c] = c < fresh ? w.fresh[i * p.columns + c] : -1;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) p.rows[t] = w.total[i];
+}
+
+// Shared memory of the plan kernels above 48 KB, once per device and kernel.
+template <class K>
+cudaError_t allow_smem(K kernel) {
+  return cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                              cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+}
+
+int64_t move_chunks(const knn_pages& p) {
+  int64_t chunks = 0;
+  for (int k = 0; k < p.n_pools; ++k)
+    chunks += (p.row_bytes[k] * p.page_rows + kMoveChunk - 1) / kMoveChunk;
+  return chunks;
+}
+
+unsigned move_grid(int64_t items) {
+  return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(items, 148 * 8)));
+}
+
+}  // namespace
+
+cudaError_t launch_pages_grow(const knn_pages& p, const int32_t* seqs, const int32_t* counts,
+                              int64_t n, int64_t total, cudaStream_t stream) {
+  const size_t smem = 4 * (n + 1 + (p.sequences + 31) / 32);
+  if (smem > 40 * 1024)
+    if (cudaError_t e = allow_smem(grow_kernel)) return e;
+  store_count_launches(1);
+  return launch_after(grow_kernel, 1, kPlanThreads, smem, stream, p, seqs, counts,
+                      static_cast<int>(n), total);
+}
+
+cudaError_t launch_pages_free(const knn_pages& p, const int32_t* seqs, int64_t n,
+                              cudaStream_t stream) {
+  store_count_launches(1);
+  return launch_after(free_kernel, static_cast<unsigned>(n), kMoveThreads, 0, stream, p, seqs,
+                      static_cast<int>(n));
+}
+
+cudaError_t launch_pages_copy(const knn_pages& p, const int32_t* sources, const int32_t* targets,
+                              int64_t n, cudaStream_t stream) {
+  const size_t smem = 4 * ((p.pages + 31) / 32);
+  if (smem > 40 * 1024)
+    if (cudaError_t e = allow_smem(copy_plan_kernel)) return e;
+  store_count_launches(2);
+  if (cudaError_t e = launch_after(copy_plan_kernel, 1, kPlanThreads, smem, stream, p, sources,
+                                   targets, n))
+    return e;
+  const int64_t chunks = move_chunks(p);
+  return launch_after(copy_kernel, move_grid(n * chunks), kMoveThreads, 0, stream, p, sources,
+                      targets, n, chunks);
+}
+
+cudaError_t launch_pages_fork(const knn_pages& p, const int32_t* parents, const int32_t* children,
+                              int64_t n, cudaStream_t stream) {
+  const size_t smem = 4 * (2 * n + (p.sequences + 31) / 32);
+  if (smem > 40 * 1024)
+    if (cudaError_t e = allow_smem(fork_plan_kernel)) return e;
+  store_count_launches(2);
+  if (cudaError_t e = launch_after(fork_plan_kernel, 1, kPlanThreads, smem, stream, p, parents,
+                                   children, static_cast<int>(n)))
+    return e;
+  const int64_t shares = (p.columns + kShareChunk - 1) / kShareChunk, chunks = move_chunks(p);
+  return launch_after(fork_kernel, move_grid(n * (shares + chunks)), kMoveThreads, 0, stream, p,
+                      parents, children, n, shares, chunks);
+}
+
+int64_t pages_compact_words(const knn_pages& p, int64_t n, int64_t keep_columns) {
+  const int64_t chunks = std::max<int64_t>(1, (keep_columns + kKeepChunk - 1) / kKeepChunk);
+  return n * (chunks + 1 + p.columns);
+}
+
+cudaError_t launch_pages_compact(const knn_pages& p, const int32_t* sources,
+                                 const int32_t* targets, int64_t n, const uint8_t* keep,
+                                 int64_t keep_columns, int64_t keep_stride, int32_t* workspace,
+                                 cudaStream_t stream) {
+  CompactWork w;
+  w.chunks = std::max<int64_t>(1, (keep_columns + kKeepChunk - 1) / kKeepChunk);
+  w.kept = workspace;
+  w.total = w.kept + n * w.chunks;
+  w.fresh = w.total + n;
+  const size_t smem = 4 * (n + (p.sequences + 31) / 32);
+  if (smem > 40 * 1024)
+    if (cudaError_t e = allow_smem(compact_plan_kernel)) return e;
+  store_count_launches(4);
+  const unsigned grid = static_cast<unsigned>(n * w.chunks);
+  if (cudaError_t e = launch_after(compact_count_kernel, grid, kKeepChunk, 0, stream, p, sources,
+                                   keep, keep_columns, keep_stride, w))
+    return e;
+  if (cudaError_t e = launch_after(compact_plan_kernel, 1, kPlanThreads, smem, stream, p, sources,
+                                   targets, static_cast<int>(n), keep_columns, w))
+    return e;
+  if (cudaError_t e = launch_after(compact_kernel, grid, kMoveThreads, 0, stream, p, sources, keep,
+                                   keep_stride, w))
+    return e;
+  return launch_after(compact_commit_kernel, static_cast<unsigned>(n), kMoveThreads, 0, stream, p,
+                      sources, targets, w);
+}
+
+}  // namespace knn

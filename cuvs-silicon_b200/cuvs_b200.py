@@ -37,6 +37,7 @@ KNN_ENOMEM = 5
 KNN_EUNSUPPORTED = 6
 DTYPE_F32 = 0
 DTYPE_F16 = 1
+DTYPE_BF16 = 2
 METRIC_L2_EXPANDED = 0
 METRIC_INNER_PRODUCT = 1
 FILE_FVECS = 0
@@ -50,6 +51,25 @@ class KnnPlan(ctypes.Structure):
         "query_block", "query_tiles", "row_tiles", "splits", "units", "grid",
         "stages", "smem_bytes", "partial_bytes", "pair", "unit_queries",
         "compact_heap")]
+
+
+PAGES_MAX_POOLS = 8
+
+
+class KnnPages(ctypes.Structure):
+    _fields_ = [("table", ctypes.c_void_p), ("rows", ctypes.c_void_p), ("refs", ctypes.c_void_p),
+                ("status", ctypes.c_void_p), ("pools", ctypes.c_void_p * PAGES_MAX_POOLS),
+                ("row_bytes", ctypes.c_int64 * PAGES_MAX_POOLS), ("sequences", ctypes.c_int64),
+                ("columns", ctypes.c_int64), ("pages", ctypes.c_int64),
+                ("page_rows", ctypes.c_int32), ("n_pools", ctypes.c_int32),
+                ("device", ctypes.c_int32)]
+
+
+class KnnQ4Rows(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("zeros", ctypes.c_void_p),
+                ("norms", ctypes.c_void_p), ("n_rows", ctypes.c_int64), ("dim", ctypes.c_int64),
+                ("group", ctypes.c_int32), ("scale_dtype", ctypes.c_int32),
+                ("device", ctypes.c_int32), ("pages", ctypes.POINTER(KnnPages))]
 
 
 _lib = None
@@ -105,6 +125,19 @@ def lib() -> ctypes.CDLL:
         "knn_index_rerank_stats": (I, [P, ctypes.POINTER(I64), ctypes.POINTER(I64)]),
         "knn_index_search_noalloc": (I, [P, P, I64, I64, P, P]),
         "knn_selftest_bounded_wait": (I, [I, I64]),
+        "knn_pages_grow": (I, [P, P, P, I64, I64, P]),
+        "knn_pages_free": (I, [P, P, I64, P]),
+        "knn_pages_copy": (I, [P, P, P, I64, P]),
+        "knn_pages_fork": (I, [P, P, P, I64, P]),
+        "knn_pages_compact_workspace": (I64, [P, I64, I64]),
+        "knn_pages_compact": (I, [P, P, P, I64, P, I64, I64, P, P]),
+        "knn_q4_row_bytes": (I64, [I64]),
+        "knn_q4_pack": (I, [P, P, I, I64, I64, I64, P]),
+        "knn_q4_append": (I, [P, P, P, I64, P, I, I64, I64, P]),
+        "knn_q4_read": (I, [P, P, P, I64, I64, I64, P, I64, P]),
+        "knn_q4_products": (I, [P, I64, I64, P, I, I64, I64, P, I, I64, P]),
+        "knn_q4_search_workspace": (I64, [I64]),
+        "knn_q4_search": (I, [P, I64, I64, P, I, I64, I64, I64, I, P, P, P, P]),
         "knn_dispatch_count": (ctypes.c_uint64, []),
         "knn_reset_dispatch_count": (None, []),
     }
@@ -326,6 +359,344 @@ class Index:
 
     def reset_kernel_stats(self) -> None:
         _check(lib().knn_index_reset_kernel_stats(self._h))
+
+
+# ---------------------------------------------------------------- row store
+# Rows in 4 bits, and pages of rows.  Everything here takes CUDA tensors of one
+# device, works on that device's current torch stream without synchronising,
+# and can be captured into a CUDA graph.
+
+PAGES_ERRORS = {1: "a sequence or page that does not exist",
+                2: "a target listed twice, or as a source too",
+                3: "a fork's child or a compaction's target holds rows",
+                4: "counts below 0, above the length, or not the total",
+                5: "more pages than the table has columns",
+                6: "too few free pages"}
+
+
+def _on_device(name, t, device, dtype=None, shape=None, dense=True):
+    """Refuses a tensor that a kernel could not take."""
+    if not getattr(t, "is_cuda", False):
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if dtype is not None and t.dtype is not dtype:
+        raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
+    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {shape}")
+    if dense and not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t
+
+
+def _list(name, t, device):
+    import torch
+
+    _on_device(name, t, device, torch.int32)
+    if t.dim() != 1:
+        raise ValueError(f"{name} must be a list of int32")
+    return t
+
+
+def _two_lists(names, a, b, device):
+    _list(names[0], a, device)
+    _list(names[1], b, device)
+    if a.shape != b.shape:
+        raise ValueError(f"{names[0]} and {names[1]} differ in length")
+
+
+def _stream(device) -> int:
+    import torch
+
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _rows_of(name, t, device, dim):
+    """A matrix of vectors (or one vector) of floats whose values lie side by side."""
+    import torch
+
+    codes = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
+    _on_device(name, t, device, dense=False)
+    if t.dtype not in codes:
+        raise ValueError(f"{name} of {t.dtype}: not float32, float16 or bfloat16")
+    if t.dim() not in (1, 2) or t.shape[-1] != dim:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, not (n, {dim})")
+    if (dim > 1 and t.stride(-1) != 1) or (t.dim() == 2 and t.shape[0] > 1 and t.stride(0) < dim):
+        raise ValueError(f"{name}: the values of a row must lie side by side, rows apart")
+    n = t.shape[0] if t.dim() == 2 else 1
+    return n, (t.stride(0) if t.dim() == 2 and n > 1 else dim), codes[t.dtype]
+
+
+class Pages:
+    """Sequences of rows in pages, over the caller's tensors (nothing is
+    copied; they stay alive with this object):
+
+    table  int32 [sequences, columns]: page numbers, -1 where there is none
+    rows   int32 [sequences]: lengths
+    refs   int32 [pages]: table entries that hold the page; 0: free
+    pools  up to 8 tensors [pages, page_rows, ...]: the rows' contents
+
+    ``Pages.empty`` makes the first three.  Lists are int32 CUDA tensors.  A
+    call that breaks a rule that only the device can see (an index out of
+    range, a target listed twice, too few free pages, ...) changes nothing and
+    leaves a note that ``check`` raises; see knn_pages_* in the C header.
+    """
+
+    def __init__(self, table, rows, refs, pools):
+        import torch
+
+        _on_device("table", table, None, torch.int32)
+        device = table.device
+        if table.dim() != 2:
+            raise ValueError("table must be 2-D")
+        _on_device("rows", rows, device, torch.int32, (table.shape[0],))
+        _on_device("refs", refs, device, torch.int32)
+        if refs.dim() != 1:
+            raise ValueError("refs must be 1-D")
+        pools = list(pools)
+        if len(pools) > PAGES_MAX_POOLS:
+            raise ValueError(f"{len(pools)} pools: at most {PAGES_MAX_POOLS}")
+        if not pools:
+            raise ValueError("at least one pool")
+        c = KnnPages(table=table.data_ptr(), rows=rows.data_ptr(), refs=refs.data_ptr())
+        for k, t in enumerate(pools):
+            _on_device(f"pool {k}", t, device)
+            if t.dim() < 2 or t.shape[0] != refs.shape[0] or t.shape[1] != pools[0].shape[1]:
+                raise ValueError(f"pool {k} has shape {tuple(t.shape)}, not (pages, page_rows, ...)")
+            c.pools[k] = t.data_ptr()
+            c.row_bytes[k] = t[0, 0].numel() * t.element_size() if t.numel() else 0
+        self.status = torch.zeros(2, dtype=torch.int32, device=device)
+        c.status = self.status.data_ptr()
+        c.sequences, c.columns = table.shape
+        c.pages, c.page_rows, c.n_pools = refs.shape[0], pools[0].shape[1], len(pools)
+        c.device = device.index
+        self.table, self.rows, self.refs, self.pools, self.device = table, rows, refs, pools, device
+        self.page_rows = int(c.page_rows)
+        self._c = c
+        self._ref = ctypes.byref(c)
+        # the C checks of sizes, once
+        _check(lib().knn_pages_free(self._ref, None, 0, None))
+
+    @classmethod
+    def empty(cls, pools, sequences: int, columns: int):
+        """A store of empty sequences over the given pools."""
+        import torch
+
+        pools = list(pools)
+        if not pools or not getattr(pools[0], "is_cuda", False):
+            raise ValueError("pools must be CUDA tensors")
+        if sequences < 1 or columns < 1:
+            raise ValueError("a store has at least one sequence and one column")
+        new = dict(dtype=torch.int32, device=pools[0].device)
+        return cls(torch.full((sequences, columns), -1, **new), torch.zeros(sequences, **new),
+                   torch.zeros(pools[0].shape[0], **new), pools)
+
+    def grow(self, seqs, counts) -> None:
+        """Room for counts[i] more rows at the end of sequence seqs[i]."""
+        _two_lists(("seqs", "counts"), seqs, counts, self.device)
+        _check(lib().knn_pages_grow(self._ref, seqs.data_ptr(), counts.data_ptr(), seqs.shape[0], -1,
+                                    _stream(self.device)))
+
+    def free(self, seqs) -> None:
+        """Empties the listed sequences."""
+        _list("seqs", seqs, self.device)
+        _check(lib().knn_pages_free(self._ref, seqs.data_ptr(), seqs.shape[0], _stream(self.device)))
+
+    def copy(self, sources, targets) -> None:
+        """Copies page sources[i] onto page targets[i] in every pool."""
+        _two_lists(("sources", "targets"), sources, targets, self.device)
+        _check(lib().knn_pages_copy(self._ref, sources.data_ptr(), targets.data_ptr(),
+                                    sources.shape[0], _stream(self.device)))
+
+    def fork(self, parents, children) -> None:
+        """Makes the empty sequences children[i] copies of parents[i]: full
+        pages are shared, a part-filled last page is copied."""
+        _two_lists(("parents", "children"), parents, children, self.device)
+        _check(lib().knn_pages_fork(self._ref, parents.data_ptr(), children.data_ptr(),
+                                    parents.shape[0], _stream(self.device)))
+
+    def compact(self, sources, targets, keep) -> None:
+        """targets[i] (empty, or sources[i] itself) becomes the rows j of
+        sources[i] with keep[i, j], in order, in fresh pages."""
+        import torch
+
+        _two_lists(("sources", "targets"), sources, targets, self.device)
+        _on_device("keep", keep, self.device, dense=False)
+        n = sources.shape[0]
+        if keep.dtype not in (torch.bool, torch.uint8) or keep.dim() != 2 or keep.shape[0] != n:
+            raise ValueError(f"keep must be bool or uint8 of shape ({n}, rows)")
+        columns = keep.shape[1]
+        stride = keep.stride(0) if n > 1 else columns
+        if (columns > 1 and keep.stride(1) != 1) or stride < columns:
+            raise ValueError("keep: the flags of a sequence must lie side by side, sequences apart")
+        work = torch.empty(max(1, lib().knn_pages_compact_workspace(self._ref, n, columns)),
+                           dtype=torch.uint8, device=self.device)
+        _check(lib().knn_pages_compact(self._ref, sources.data_ptr(), targets.data_ptr(), n,
+                                       keep.data_ptr(), columns, stride, work.data_ptr(),
+                                       _stream(self.device)))
+
+    def check(self) -> None:
+        """Waits for the store's calls; raises the first error that one of
+        them found (and forgets it)."""
+        error = int(self.status[0].item())
+        if error:
+            self.status[0] = 0
+            raise ValueError(f"row store: {PAGES_ERRORS.get(error, error)}")
+
+
+class Q4Rows:
+    """Rows in 4 bits, over the caller's tensors:
+
+    codes   uint8 [n, 16 * ceil(dim / 32)], two codes a byte, the first low
+    scales  float16 or bfloat16 [n, ceil(dim / group)], group 32, 64 or 128
+    zeros   uint8 like scales, or None: 8 throughout
+    norms   float32 [n], |row|^2, or None (only needed to search by L2)
+
+    ``value = (code - zero) * scale``.  With ``pages`` the tensors are pools
+    [pages, page_rows, ...] of that store and calls name a sequence.
+    """
+
+    def __init__(self, codes, scales, dim: int, group: int, zeros=None, norms=None, pages=None):
+        import torch
+
+        _on_device("codes", codes, None, torch.uint8)
+        device, lead = codes.device, tuple(codes.shape[:-1])
+        if dim < 1 or group not in (32, 64, 128):
+            raise ValueError(f"rows of {dim} values in groups of {group}")
+        groups, width = -(-dim // group), 16 * (-(-dim // 32))
+        if pages is not None and lead != (pages.refs.shape[0], pages.page_rows):
+            raise ValueError(f"codes have shape {tuple(codes.shape)}, not (pages, page_rows, {width})")
+        if pages is None and len(lead) != 1:
+            raise ValueError(f"codes have shape {tuple(codes.shape)}, not (n, {width})")
+        if pages is not None and pages.device != device:
+            raise ValueError(f"the pages are on {pages.device}, the codes on {device}")
+        _on_device("codes", codes, device, torch.uint8, lead + (width,))
+        _on_device("scales", scales, device, None, lead + (groups,))
+        if scales.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"scales of {scales.dtype}: not float16 or bfloat16")
+        if zeros is not None:
+            _on_device("zeros", zeros, device, torch.uint8, lead + (groups,))
+        if norms is not None:
+            _on_device("norms", norms, device, torch.float32, lead)
+        c = KnnQ4Rows(codes=codes.data_ptr(), scales=scales.data_ptr(), dim=dim, group=group,
+                      device=device.index)
+        c.zeros = zeros.data_ptr() if zeros is not None else None
+        c.norms = norms.data_ptr() if norms is not None else None
+        c.scale_dtype = DTYPE_F16 if scales.dtype is torch.float16 else DTYPE_BF16
+        c.n_rows = lead[0] if pages is None else lead[0] * lead[1]
+        if pages is not None:
+            c.pages = ctypes.pointer(pages._c)
+        self.codes, self.scales, self.zeros, self.norms, self.pages = codes, scales, zeros, norms, pages
+        self.dim, self.group, self.device, self.n_rows = dim, group, device, int(c.n_rows)
+        self._c = c
+        self._ref = ctypes.byref(c)
+        # the C checks of sizes, once
+        _check(lib().knn_q4_products(self._ref, -1 if pages is None else 0, 0, None, 0, 0, 0, None, 0,
+                                     0, None))
+
+    def _range(self, seq, count):
+        if self.pages is None:
+            if seq is not None:
+                raise ValueError("dense rows have no sequences")
+            return -1, self.n_rows if count is None else count
+        if seq is None or count is None:
+            raise ValueError("rows in pages need seq and count")
+        return seq, count
+
+    def append(self, seqs, counts, rows) -> None:
+        """Quantises ``rows``, counts[i] of them for the end of seqs[i], those
+        of seqs[0] first (Pages.grow, then the rows)."""
+        if self.pages is None:
+            raise ValueError("dense rows do not grow")
+        _two_lists(("seqs", "counts"), seqs, counts, self.device)
+        n, ld, dtype = _rows_of("rows", rows, self.device, self.dim)
+        _check(lib().knn_q4_append(self._ref, seqs.data_ptr(), counts.data_ptr(), seqs.shape[0],
+                                   rows.data_ptr(), dtype, n, ld, _stream(self.device)))
+
+    def read(self, seqs=None, counts=None, total=None, first: int = 0):
+        """The values of rows, float32: rows first .. first + total - 1 of dense
+        rows, or the last counts[i] rows of seqs[i], ``total`` in all."""
+        import torch
+
+        if self.pages is None:
+            if seqs is not None or counts is not None:
+                raise ValueError("dense rows have no sequences")
+            total = self.n_rows - first if total is None else total
+            if total < 0:
+                raise ValueError(f"{total} rows")
+            out = torch.empty((total, self.dim), dtype=torch.float32, device=self.device)
+            _check(lib().knn_q4_read(self._ref, None, None, 0, first, total, out.data_ptr(), self.dim,
+                                     _stream(self.device)))
+            return out
+        if seqs is None or counts is None or total is None or total < 0:
+            raise ValueError("rows in pages need seqs, counts and their total")
+        _two_lists(("seqs", "counts"), seqs, counts, self.device)
+        out = torch.empty((total, self.dim), dtype=torch.float32, device=self.device)
+        _check(lib().knn_q4_read(self._ref, seqs.data_ptr(), counts.data_ptr(), seqs.shape[0], first,
+                                 total, out.data_ptr(), self.dim, _stream(self.device)))
+        return out
+
+    def products(self, x, seq=None, count=None, out=None, dtype=None):
+        """x [batch, dim] (or one vector) times rows 0 .. count - 1: [batch,
+        count] in ``dtype`` (float32 unless given).  In pages: of sequence
+        ``seq``, 0 beyond its length."""
+        import torch
+
+        seq, count = self._range(seq, count)
+        n, ldx, code = _rows_of("x", x, self.device, self.dim)
+        if count < 0 or count > self.n_rows:
+            raise ValueError(f"{count} of {self.n_rows} rows")
+        shape = (n, count) if x.dim() == 2 else (count,)
+        if out is None:
+            out = torch.empty(shape, dtype=dtype or torch.float32, device=self.device)
+        elif dtype is not None and out.dtype is not dtype:
+            raise ValueError(f"out is {out.dtype}, not {dtype}")
+        elif tuple(out.shape) != shape:
+            raise ValueError(f"out has shape {tuple(out.shape)}, not {shape}")
+        _, ldo, out_code = _rows_of("out", out, self.device, count)
+        _check(lib().knn_q4_products(self._ref, seq, count, x.data_ptr(), code, n, ldx, out.data_ptr(),
+                                     out_code, ldo, _stream(self.device)))
+        return out
+
+    def search(self, queries, k: int, metric: int = METRIC_L2_EXPANDED, seq=None, count=None):
+        """The k nearest rows of each query: (neighbors int64, distances
+        float32), as Index.search orders and pads them."""
+        import torch
+
+        seq, count = self._range(seq, count)
+        n, ld, code = _rows_of("queries", queries, self.device, self.dim)
+        if queries.dim() != 2:
+            raise ValueError("queries must be 2-D")
+        if k < 1 or k > MAX_K:
+            raise ValueError(f"k = {k}: 1 to {MAX_K}")
+        if count < 0 or count > self.n_rows:
+            raise ValueError(f"{count} of {self.n_rows} rows")
+        neighbors = torch.empty((n, k), dtype=torch.int64, device=self.device)
+        distances = torch.empty((n, k), dtype=torch.float32, device=self.device)
+        work = torch.empty(lib().knn_q4_search_workspace(count), dtype=torch.uint8, device=self.device)
+        _check(lib().knn_q4_search(self._ref, seq, count, queries.data_ptr(), code, n, ld, k, metric,
+                                   neighbors.data_ptr(), distances.data_ptr(), work.data_ptr(),
+                                   _stream(self.device)))
+        return neighbors, distances
+
+
+def q4_pack(rows, group: int = 64, zero_points: bool = False, scale_dtype=None) -> Q4Rows:
+    """Quantises rows [n, dim] (float32, float16 or bfloat16) to 4 bits with a
+    scale (float16 unless ``scale_dtype`` says bfloat16), and where asked a
+    zero point, for every ``group`` values; see knn_q4_pack in the C header."""
+    import torch
+
+    if getattr(rows, "ndim", 0) != 2 or rows.shape[1] < 1 or group not in (32, 64, 128):
+        raise ValueError("rows must be 2-D, in groups of 32, 64 or 128")
+    n, dim = rows.shape
+    _, ld, code = _rows_of("rows", rows, rows.device, dim)
+    groups, new = -(-dim // group), dict(device=rows.device)
+    out = Q4Rows(torch.empty((n, 16 * (-(-dim // 32))), dtype=torch.uint8, **new),
+                 torch.empty((n, groups), dtype=scale_dtype or torch.float16, **new), dim, group,
+                 torch.empty((n, groups), dtype=torch.uint8, **new) if zero_points else None,
+                 torch.empty(n, dtype=torch.float32, **new))
+    _check(lib().knn_q4_pack(out._ref, rows.data_ptr(), code, n, ld, 0, _stream(out.device)))
+    return out
 
 
 # ------------------------------------------------------------ dataset files

@@ -58,6 +58,7 @@ extern "C" {
 
 #define KNN_DTYPE_F32 0
 #define KNN_DTYPE_F16 1
+#define KNN_DTYPE_BF16 2 /* row store only */
 
 /* Metrics.  L2Expanded: squared L2 distances, ascending.  InnerProduct
  * (declared by the reference at include/cuvs/distance/distance.hpp:5-8 and
@@ -357,6 +358,162 @@ int knn_index_reset_kernel_stats(knn_index* index);
  * KNN_ETIMEOUT when the wait gave up and reported it, as designed; the
  * device stays usable.  No counterpart in the reference. */
 int knn_selftest_bounded_wait(int device, int64_t limit_us);
+
+/* ------------------------------------------------------------------------
+ * Row store: rows in 4 bits, and pages of rows that can grow, be shared, be
+ * compacted and be freed.  No counterpart in the reference, whose index is
+ * frozen (its FAISS adapter builds it again for every add,
+ * tests/faiss_v1_8_cagra_runtime_smoke.cpp:148-171).
+ *
+ * These functions keep nothing between calls: the caller owns every buffer.
+ * All pointers, except the two descriptors themselves, are memory of the
+ * descriptor's device; nothing is staged, classified or allocated.  They
+ * enqueue on `cuda_stream` (NULL: the legacy default stream) of that device,
+ * return without synchronising, may be captured into a CUDA graph and leave
+ * the calling thread's current device as it was.  Calls that read and change
+ * the same store must be ordered by the caller (one stream, or events).
+ * ------------------------------------------------------------------------ */
+
+#define KNN_PAGES_MAX_POOLS 8
+#define KNN_PAGES_MAX_LIST 4096            /* sequences of one call */
+#define KNN_PAGES_MAX_PAGES (1 << 20)      /* pages of a store */
+#define KNN_PAGES_MAX_SEQUENCES (1 << 20)  /* sequences of a store */
+
+/* A store of rows in pages.  Row j of sequence s lies in page
+ * table[s * columns + j / page_rows], slot j % page_rows, of every pool;
+ * pools share the page numbers.  refs[p] counts the table entries that hold
+ * page p; a page without any is free.  Table entries at and beyond
+ * ceil(rows[s] / page_rows) are -1.  A new store has table = -1 and rows =
+ * refs = 0 throughout. */
+typedef struct knn_pages {
+  int32_t* table;      /* [sequences][columns] */
+  int32_t* rows;       /* [sequences]: lengths */
+  int32_t* refs;       /* [pages] */
+  int32_t* status;     /* [2]: first error (0 = none), last change applied */
+  void* pools[KNN_PAGES_MAX_POOLS]; /* [pages][page_rows][row_bytes[k]] each */
+  int64_t row_bytes[KNN_PAGES_MAX_POOLS]; /* 1 .. 2^24 each */
+  int64_t sequences, columns, pages;
+  int32_t page_rows;
+  int32_t n_pools;
+  int32_t device;
+} knn_pages;
+
+/* What a kernel found wrong with a call (status[0]).  Such a call changes
+ * nothing but the status; later calls run as usual.  status[0] keeps the
+ * first error until the caller writes 0. */
+#define KNN_PAGES_OUT_OF_RANGE 1 /* a sequence or page that does not exist */
+#define KNN_PAGES_LISTED_TWICE 2 /* a target listed twice, or as a source too */
+#define KNN_PAGES_NOT_EMPTY 3    /* a fork's child or a compaction's target holds rows */
+#define KNN_PAGES_BAD_COUNT 4    /* counts below 0, above the length, or not the total */
+#define KNN_PAGES_TOO_LONG 5     /* more pages than the table has columns */
+#define KNN_PAGES_NONE_FREE 6    /* too few free pages */
+
+/* Room for counts[i] more rows at the end of sequence seqs[i] (each listed
+ * once; n <= KNN_PAGES_MAX_LIST).  Fresh pages are the lowest-numbered free
+ * ones, given out in the order of the list.  The rows' contents are what the
+ * pages held.  total: the counts' sum where the caller knows it (checked),
+ * or -1. */
+int knn_pages_grow(const knn_pages* pages, const int32_t* seqs, const int32_t* counts,
+                   int64_t n, int64_t total, void* cuda_stream);
+
+/* Empties the listed sequences: their pages lose a reference each, their
+ * table rows become -1 and their lengths 0.  A sequence may be empty already,
+ * or be listed again. */
+int knn_pages_free(const knn_pages* pages, const int32_t* seqs, int64_t n, void* cuda_stream);
+
+/* Copies page sources[i] onto page targets[i] in every pool, i < n <=
+ * KNN_PAGES_MAX_PAGES.  Targets differ from one another and from every
+ * source.  Table, lengths and references stay as they are. */
+int knn_pages_copy(const knn_pages* pages, const int32_t* sources, const int32_t* targets,
+                   int64_t n, void* cuda_stream);
+
+/* Makes children[i], an empty sequence, a copy of parents[i]: it shares the
+ * parent's full pages and gets a fresh page with the rows of a last page that
+ * is not full, so that both can grow.  A parent may be listed more than once;
+ * parents are read as they were before the call. */
+int knn_pages_fork(const knn_pages* pages, const int32_t* parents, const int32_t* children,
+                   int64_t n, void* cuda_stream);
+
+/* targets[i] becomes the rows j of sources[i] with keep[i * keep_stride + j]
+ * != 0, in their order, in fresh pages; no source may be longer than
+ * keep_columns.  A target is an empty sequence, or the source itself, whose
+ * old pages then lose a reference.  The fresh pages have to be free before
+ * the call.  workspace: knn_pages_compact_workspace bytes of device memory
+ * (16-byte aligned), which this call alone uses until it is done. */
+int64_t knn_pages_compact_workspace(const knn_pages* pages, int64_t n, int64_t keep_columns);
+int knn_pages_compact(const knn_pages* pages, const int32_t* sources, const int32_t* targets,
+                      int64_t n, const uint8_t* keep, int64_t keep_columns, int64_t keep_stride,
+                      void* workspace, void* cuda_stream);
+
+/* Rows in 4 bits: value j of a row is (code - zero) * scale, with a scale and
+ * a zero point for every `group` values.  A row's codes take
+ * knn_q4_row_bytes(dim) = 16 * ceil(dim / 32) bytes, two to a byte, the first
+ * in the low four bits; codes behind the last value count for nothing.
+ * pages == NULL: n_rows rows one after another.  Otherwise the buffers are
+ * pools of that store (n_rows = pages * page_rows), and `pages` has to live
+ * as long as the call. */
+typedef struct knn_q4_rows {
+  uint8_t* codes;  /* [n_rows][16 * ceil(dim / 32)], 16-byte aligned */
+  void* scales;    /* [n_rows][ceil(dim / group)], fp16 or bf16 */
+  uint8_t* zeros;  /* [n_rows][ceil(dim / group)], 0 .. 15, or NULL: 8 throughout */
+  float* norms;    /* [n_rows]: |row|^2, or NULL */
+  int64_t n_rows;
+  int64_t dim;         /* 1 .. KNN_Q4_MAX_DIM */
+  int32_t group;       /* 32, 64 or 128 */
+  int32_t scale_dtype; /* KNN_DTYPE_F16 or KNN_DTYPE_BF16 */
+  int32_t device;
+  const knn_pages* pages;
+} knn_q4_rows;
+
+#define KNN_Q4_MAX_DIM 65536
+int64_t knn_q4_row_bytes(int64_t dim);
+
+/* Quantises n rows (row i at rows + i * ld values, of type dtype: F32, F16 or
+ * BF16) into rows first .. first + n - 1 of dense 4-bit rows.
+ *   zeros == NULL: scale = max|v| / 7, code = v / scale + 8
+ *   otherwise:     scale = (high - low) / 15, zero = -low / scale,
+ *                  code = v / scale + zero, low = min(0, min v), high = max(0, max v)
+ * The scale is rounded to 32 bits and then to its type; quotients go to the
+ * nearest whole number, ties to even (exactly), and codes are clamped to
+ * 0 .. 15.  A group that holds a NaN or an infinity, or whose scale
+ * overflows, reads as NaN; one whose scale rounds to 0 reads as 0. */
+int knn_q4_pack(const knn_q4_rows* q4, const void* rows, int dtype, int64_t n, int64_t ld,
+                int64_t first, void* cuda_stream);
+
+/* knn_pages_grow, and the new rows: `total` rows, those of seqs[0] first. */
+int knn_q4_append(const knn_q4_rows* q4, const int32_t* seqs, const int32_t* counts, int64_t n,
+                  const void* rows, int dtype, int64_t total, int64_t ld, void* cuda_stream);
+
+/* The values of rows, fp32, row i at out + i * ld.  Dense rows: seqs =
+ * counts = NULL, rows first .. first + total - 1.  In pages: the last
+ * counts[i] rows of seqs[i], one sequence after another, `total` in all
+ * (first = 0); a list that is wrong sets status[0] and writes nothing. */
+int knn_q4_read(const knn_q4_rows* q4, const int32_t* seqs, const int32_t* counts, int64_t n,
+                int64_t first, int64_t total, float* out, int64_t ld, void* cuda_stream);
+
+/* Products of `batch` vectors (vector b at x + b * ldx) with rows 0 .. count
+ * - 1: out[b * ldo + i] = row i . x_b, summed in fp32 and rounded once to
+ * out_dtype.  In pages: rows of sequence `seq`; beyond its length 0 is
+ * written, and a row whose page is missing gives NaN.  Dense rows: seq = -1. */
+int knn_q4_products(const knn_q4_rows* q4, int64_t seq, int64_t count, const void* x, int dtype,
+                    int64_t batch, int64_t ldx, void* out, int out_dtype, int64_t ldo,
+                    void* cuda_stream);
+
+/* The k (1 .. KNN_MAX_K) nearest of the rows that knn_q4_products would
+ * multiply, for each of n_queries queries: squared L2 distances to the rows'
+ * 4-bit values, ascending, or inner products, descending; ties by ascending
+ * index; -1 and +inf (-inf) where there are fewer.  The k + 16 best rows by
+ * fp32 sums are found first and then ordered by distances summed in 64 bits,
+ * which are returned rounded to fp32: the result is the exact one unless 16
+ * rows or more lie within fp32's rounding (for L2, of |row|^2 - 2 q.row) at
+ * the k-th place.  A row whose distance is no finite number is no
+ * neighbour.  L2 needs the norms.  workspace: knn_q4_search_workspace bytes
+ * of device memory (16-byte aligned), which this call alone uses until it is
+ * done. */
+int64_t knn_q4_search_workspace(int64_t count);
+int knn_q4_search(const knn_q4_rows* q4, int64_t seq, int64_t count, const void* queries,
+                  int dtype, int64_t n_queries, int64_t ld, int64_t k, int metric,
+                  int64_t* neighbors, float* distances, void* workspace, void* cuda_stream);
 
 /* Number of engine kernels launched since the last reset (all indices).
  * Replaces cagra::metal_dispatch_count (cagra.hpp:119-122). */
