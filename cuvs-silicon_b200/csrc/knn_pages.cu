@@ -627,12 +627,7 @@ __global__ void __launch_bounds__(kMoveThreads) compact_commit_kernel(knn_pages 
   if (threadIdx.x == 0) p.rows[t] = w.total[i];
 }
 
-// Shared memory of the plan kernels above 48 KB, once per device and kernel.
-template <class K>
-cudaError_t allow_smem(K kernel) {
-  return cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                              cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-}
+constexpr int kPlanSmem = 200 * 1024;  // at most: a bitmap of 2^20 bits and lists of 2 x 4096
 
 int64_t move_chunks(const knn_pages& p) {
   int64_t chunks = 0;
@@ -650,8 +645,9 @@ unsigned move_grid(int64_t items) {
 cudaError_t launch_pages_grow(const knn_pages& p, const int32_t* seqs, const int32_t* counts,
                               int64_t n, int64_t total, cudaStream_t stream) {
   const size_t smem = 4 * (n + 1 + (p.sequences + 31) / 32);
+  static std::atomic<uint64_t> allowed{0};
   if (smem > 40 * 1024)
-    if (cudaError_t e = allow_smem(grow_kernel)) return e;
+    if (cudaError_t e = allow_smem(grow_kernel, kPlanSmem, &allowed)) return e;
   store_count_launches(1);
   return launch_after(grow_kernel, 1, kPlanThreads, smem, stream, p, seqs, counts,
                       static_cast<int>(n), total);
@@ -667,8 +663,9 @@ cudaError_t launch_pages_free(const knn_pages& p, const int32_t* seqs, int64_t n
 cudaError_t launch_pages_copy(const knn_pages& p, const int32_t* sources, const int32_t* targets,
                               int64_t n, cudaStream_t stream) {
   const size_t smem = 4 * ((p.pages + 31) / 32);
+  static std::atomic<uint64_t> allowed{0};
   if (smem > 40 * 1024)
-    if (cudaError_t e = allow_smem(copy_plan_kernel)) return e;
+    if (cudaError_t e = allow_smem(copy_plan_kernel, kPlanSmem, &allowed)) return e;
   store_count_launches(2);
   if (cudaError_t e = launch_after(copy_plan_kernel, 1, kPlanThreads, smem, stream, p, sources,
                                    targets, n))
@@ -681,8 +678,9 @@ cudaError_t launch_pages_copy(const knn_pages& p, const int32_t* sources, const 
 cudaError_t launch_pages_fork(const knn_pages& p, const int32_t* parents, const int32_t* children,
                               int64_t n, cudaStream_t stream) {
   const size_t smem = 4 * (2 * n + (p.sequences + 31) / 32);
+  static std::atomic<uint64_t> allowed{0};
   if (smem > 40 * 1024)
-    if (cudaError_t e = allow_smem(fork_plan_kernel)) return e;
+    if (cudaError_t e = allow_smem(fork_plan_kernel, kPlanSmem, &allowed)) return e;
   store_count_launches(2);
   if (cudaError_t e = launch_after(fork_plan_kernel, 1, kPlanThreads, smem, stream, p, parents,
                                    children, static_cast<int>(n)))
@@ -707,8 +705,9 @@ cudaError_t launch_pages_compact(const knn_pages& p, const int32_t* sources,
   w.total = w.kept + n * w.chunks;
   w.fresh = w.total + n;
   const size_t smem = 4 * (n + (p.sequences + 31) / 32);
+  static std::atomic<uint64_t> allowed{0};
   if (smem > 40 * 1024)
-    if (cudaError_t e = allow_smem(compact_plan_kernel)) return e;
+    if (cudaError_t e = allow_smem(compact_plan_kernel, kPlanSmem, &allowed)) return e;
   store_count_launches(4);
   const unsigned grid = static_cast<unsigned>(n * w.chunks);
   if (cudaError_t e = launch_after(compact_count_kernel, grid, kKeepChunk, 0, stream, p, sources,

@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "knn_q4.h"
 
@@ -32,7 +33,7 @@ __device__ __forceinline__ float scale_of(const Q4View& v, int64_t row, int g) {
                       : __half2float(__ushort_as_half(bits));
 }
 __device__ __forceinline__ int zero_of(const Q4View& v, int64_t row, int g) {
-  return v.zeros ? v.zeros[row * v.groups + g] : 8;
+  return v.zeros ? v.zeros[row * v.groups + g] & 15 : 8;
 }
 
 // The larger of two numbers, NaN where either is one.
@@ -263,66 +264,6 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Q4View v, Q4List l, floa
 // the order does not depend on |q|^2).
 enum { kStore = 0, kKeyL2 = 1, kKeyProduct = 2 };
 
-struct Q4Out {
-  void* y;
-  int dtype;
-  int64_t ld;
-  int mode;
-};
-
-__device__ __forceinline__ void put(const Q4Out& o, int64_t b, int64_t i, float y, float norm) {
-  if (o.mode == kKeyL2) y = norm - 2.0f * y;
-  if (o.mode == kKeyProduct) y = -y;
-  const int64_t at = b * o.ld + i;
-  if (o.dtype == KNN_DTYPE_F32) static_cast<float*>(o.y)[at] = y;
-  else if (o.dtype == KNN_DTYPE_F16) static_cast<__half*>(o.y)[at] = __float2half_rn(y);
-  else static_cast<__nv_bfloat16*>(o.y)[at] = __float2bfloat16_rn(y);
-}
-
-// One warp a row, a lane 32 codes at a time.
-template <class T>
-__global__ void __launch_bounds__(kThreads) products_kernel(Q4View v, Q4Range r, const T* x,
-                                                            int64_t batch, int64_t ldx, Q4Out o) {
-  wait_for_stream();
-  int64_t n = r.count;
-  if (r.length) n = *r.length < n ? *r.length : n;
-  const int lane = threadIdx.x & 31;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); i < r.count;
-       i += static_cast<int64_t>(gridDim.x) * kWarps) {
-    const int64_t row = i < n ? v.places.at(r.seq, i) : -1;
-    for (int64_t b = 0; b < batch; ++b) {
-      float sum = 0.0f;
-      for (int c = lane; row >= 0 && c < v.width / 16; c += 32) {
-        const uint4 w = *reinterpret_cast<const uint4*>(v.codes + row * v.width + 16 * c);
-        const int g = 32 * c / v.group;
-        const float z = static_cast<float>(zero_of(v, row, g));
-        float part = 0.0f;
-        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const int64_t j = 32 * c + e;
-          if (j < v.dim)
-            part += (static_cast<float>((words[e / 8] >> (4 * (e % 8))) & 15) - z) *
-                    load_value(x + b * ldx + j);
-        }
-        sum += scale_of(v, row, g) * part;
-      }
-#pragma unroll
-      for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      if (row < 0) sum = i < n ? __int_as_float(0x7fc00000) : 0.0f;
-      if (lane == 0) put(o, b, i, sum, o.mode == kKeyL2 && row >= 0 ? v.norms[row] : 0.0f);
-    }
-  }
-}
-
-// ----------------------------------------------------------------- search
-constexpr int kGroupRows = 128;    // rows whose smallest key is kept
-constexpr int kSelectThreads = 1024;
-constexpr int kMoreCandidates = 16;  // scored again beyond the k asked for
-constexpr int kMaxCandidates = KNN_MAX_K + kMoreCandidates;
-constexpr int kGroupCap = 1024;
-constexpr int kCandCap = 4096;
-
 // Keys in an order that unsigned numbers have; a key that is +inf or NaN
 // belongs to no neighbour.
 __device__ __forceinline__ uint32_t ordered(float key) {
@@ -331,26 +272,494 @@ __device__ __forceinline__ uint32_t ordered(float key) {
   return (b >> 31) ? ~b : b | 0x80000000u;
 }
 
-// The smallest key of every kGroupRows rows.
-__global__ void __launch_bounds__(kThreads) group_min_kernel(Q4Range r, const float* keys,
-                                                             int64_t ld, uint32_t* minima,
-                                                             int64_t groups) {
+struct Q4Out {
+  void* y;
+  int dtype;
+  int64_t ld;
+  int mode;
+  uint32_t* minima;  // [vectors][tiles of 32 rows]: smallest key, or nullptr
+};
+
+// Stores a product, or makes it a key, which it stores and returns.
+__device__ __forceinline__ float put(const Q4Out& o, int64_t b, int64_t i, float y, float norm) {
+  if (o.mode == kKeyL2) y = norm - 2.0f * y;
+  if (o.mode == kKeyProduct) y = -y;
+  const int64_t at = b * o.ld + i;
+  if (o.dtype == KNN_DTYPE_F32) static_cast<float*>(o.y)[at] = y;
+  else if (o.dtype == KNN_DTYPE_F16) static_cast<__half*>(o.y)[at] = __float2half_rn(y);
+  else static_cast<__nv_bfloat16*>(o.y)[at] = __float2bfloat16_rn(y);
+  return y;
+}
+
+// The products run on the warp's own matrix instructions (mma.sync, fp16 in,
+// fp32 sums): a row's partial sums have to be scaled after every 32 to 128
+// values, which in registers is one multiply-add to a sum, while sums in
+// tensor memory would have to be read out and scaled that often, and scales
+// multiplied into the weights would no longer be exact in 16 bits.  A code
+// less its zero point is a whole number of at most 5 bits, so every product
+// in the matrix unit is exact, and the rounding is that of fp32 sums.
+//
+// Vectors become fp16 on the way into shared memory.  fp16 ones are taken as
+// they are; bf16 and fp32 ones are first scaled, each vector by a power of
+// two of its own that brings its largest finite magnitude to 2^14 .. 2^15,
+// and fp32 ones split into two fp16 parts (columns of their own, added up
+// after the group's scaling): x = high + low is off by at most 2^-24 |x| +
+// 2^-40 max|x|, a bf16 one by 2^-40 max|x| at the very most.
+//
+// A warp takes tiles of 32 rows and runs down their codes in stages of 128,
+// which it copies ahead into a ring of its own in shared memory (cp.async, no
+// barrier between warps); the ring also hands the codes of a group to the
+// lanes that the matrix instruction wants them in.  The order of the values
+// within a group is free as long as codes and vector agree, so codes are
+// unpacked where they lie:
+//   word of 8 codes, & 0x000f000f | 0x64006400 = (1024 + c0, 1024 + c4) in
+//   fp16, & 0x00f000f0 likewise (1024 + 16 c1, 1024 + 16 c5), and both again
+//   8 bits further; one fp16 instruction takes off 1024 + zero (and the 16).
+// Rows are few where the matrix is small or wide: the codes of a tile are
+// then split over 2 to 16 warps of the block (`split`) and their sums added
+// up through shared memory, in order.
+constexpr int kMmaWarps = 16;
+constexpr int kMmaThreads = 32 * kMmaWarps;
+constexpr int kTileRows4 = 32;  // rows of a tile
+constexpr int kStageCodes = 128;
+constexpr int kStageBytes4 = kTileRows4 * kStageCodes / 2;
+constexpr int kRing = 3;
+constexpr int kSumStride = 36;  // floats from column to column of a tile's sums: no bank twice
+
+struct MmaPlan {
+  int64_t tiles;
+  int32_t iterations;    // tiles that a warp's slot goes through
+  int32_t stages;        // of 128 codes in a row
+  int32_t chunk_stages;  // stages whose share of the vectors fits in shared memory
+  int32_t chunks;
+  int32_t split;  // warps that share a tile
+};
+
+struct MmaShared {
+  // ring[warp][slot][kStageBytes4], then rows[warp][slot][32], then sums
+  // (where split > 1) [warp][columns][kSumStride], then vectors
+  uint32_t largest[kQ4SearchBatch];
+  float factor[kQ4SearchBatch], inverse[kQ4SearchBatch];
+  int32_t tile_rows[kMmaWarps][kTileRows4];
+};
+
+__device__ __forceinline__ void copy_ahead(void* to, const void* from, bool valid) {
+  const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+  const int size = valid ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(from),
+               "r"(size)
+               : "memory");
+}
+__device__ __forceinline__ void copy_close() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int kLeft>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+}
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                          uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
+  const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t sixteenth2(uint32_t a, uint32_t c) {
+  const uint32_t s = 0x2c002c00u;  // 1/16
+  const __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<const __half2*>(&s),
+                            *reinterpret_cast<__half2*>(&c));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// Which 16 bytes of a row's 64 in a stage lie where: rows 0 .. 7 put them at
+// chunk ^ swizzle(row), so that the three ways below to read them (4, 8 or 16
+// bytes a lane) meet no bank twice.
+__device__ __forceinline__ int swizzle(int row) { return (row & 2) | ((row >> 2) & 1); }
+
+// A warp's place in its work: tile after tile, in each chunk after chunk, in
+// each the stages of its part.
+struct Cursor {
+  int32_t iteration, chunk, stage, end;
+  __device__ __forceinline__ void enter(const MmaPlan& p, int part) {
+    const int first = chunk * p.chunk_stages;
+    int len = p.stages - first;
+    if (len > p.chunk_stages) len = p.chunk_stages;
+    stage = first + part * len / p.split;
+    end = first + (part + 1) * len / p.split;
+  }
+  // To the next stage; true where a new tile begins.
+  __device__ __forceinline__ bool advance(const MmaPlan& p, int part) {
+    bool fresh = false;
+    ++stage;
+    while (stage >= end && iteration < p.iterations) {
+      if (++chunk == p.chunks) {
+        chunk = 0;
+        ++iteration;
+        fresh = true;
+      }
+      enter(p, part);
+    }
+    return fresh;
+  }
+};
+
+// kCols: columns of the matrix instruction in tiles of 8 (kTiles of them);
+// kParts: fp16 parts of a vector.  With kTiles = 1 and two parts, columns 0-3
+// hold the high parts of 4 vectors and 4-7 the low ones; otherwise the tiles'
+// first half holds the high parts.  kGroups: groups in a stage (128 / group).
+template <class T, int kTiles, int kParts, int kGroups, bool kZeros>
+__global__ void __launch_bounds__(kMmaThreads, 1)
+    products_kernel(Q4View v, Q4Range r, const T* x, int batch, int64_t ldx, Q4Out o, MmaPlan p) {
+  constexpr bool kPacked = kTiles == 1 && kParts == 2;
+  constexpr int kOutTiles = kPacked ? 1 : kTiles / kParts;
+  constexpr int kOutCols = 8 * kOutTiles;
+  constexpr int kPerGroup = 4 / kGroups;  // words of 8 codes a lane has in a group
+  extern __shared__ __align__(16) uint8_t raw[];
+  __shared__ MmaShared sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  uint8_t* ring = raw + warp * (kRing * kStageBytes4);
+  int32_t* ring_rows = reinterpret_cast<int32_t*>(raw + kMmaWarps * kRing * kStageBytes4) +
+                       warp * (kRing * kTileRows4);
+  float* sums = reinterpret_cast<float*>(raw + kMmaWarps * kRing * (kStageBytes4 + 4 * kTileRows4));
+  uint4* vectors = reinterpret_cast<uint4*>(
+      reinterpret_cast<uint8_t*>(sums) +
+      (p.split > 1 ? kMmaWarps * kOutCols * kSumStride * sizeof(float) : 0));
+  const int slots = kMmaWarps / p.split, slot = warp / p.split, part = warp % p.split;
+
+  if (threadIdx.x < kQ4SearchBatch) sh.largest[threadIdx.x] = 0;
   wait_for_stream();
   int64_t n = r.count;
   if (r.length) n = *r.length < n ? *r.length : n;
-  const int lane = threadIdx.x & 31;
-  const int64_t b = blockIdx.y;
-  const int64_t g = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  if (g >= groups) return;
-  uint32_t m = kNoKey;
+
+  auto tile_of = [&](int iteration) {
+    return (static_cast<int64_t>(iteration) * slots + slot) * gridDim.x + blockIdx.x;
+  };
+  // this lane's row of a tile, as a row number in the pools; -1: none
+  auto row_of = [&](int iteration) -> int32_t {
+    const int64_t i = tile_of(iteration) * kTileRows4 + lane;
+    return i < n ? static_cast<int32_t>(v.places.at(r.seq, i)) : -1;
+  };
+
+  // ---- copying codes ahead
+  Cursor ahead = {0, 0, 0, 0};
+  ahead.enter(p, part);
+  int32_t row = row_of(0), row_next = row_of(1);
+  auto send = [&](int slot_of_ring) {
+    if (ahead.iteration < p.iterations) {
+      uint8_t* to = ring + slot_of_ring * kStageBytes4;
+      const int c = 4 * ahead.stage + t;
 #pragma unroll
-  for (int j = 0; j < kGroupRows / 32; ++j) {
-    const int64_t i = g * kGroupRows + j * 32 + lane;
-    if (i < n) m = min(m, ordered(keys[b * ld + i]));
+      for (int i = 0; i < 4; ++i) {
+        const int32_t at = __shfl_sync(0xffffffffu, row, g + 8 * i);
+        const bool valid = at >= 0 && 16 * c < v.width;
+        const uint8_t* from = v.codes + (valid ? static_cast<int64_t>(at) * v.width + 16 * c : 0);
+        copy_ahead(to + (g + 8 * i) * 64 + ((t ^ swizzle(g)) << 4), from, valid);
+      }
+      ring_rows[slot_of_ring * kTileRows4 + lane] = row;
+      if (ahead.advance(p, part)) {
+        row = row_next;
+        row_next = row_of(ahead.iteration + 1);
+      }
+    }
+    copy_close();
+  };
+#pragma unroll
+  for (int j = 0; j < kRing - 1; ++j) send(j);
+
+  // ---- the vectors' scales
+  if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
+    if (threadIdx.x < kQ4SearchBatch) sh.factor[threadIdx.x] = sh.inverse[threadIdx.x] = 1.0f;
+    __syncthreads();
+  } else {
+    __syncthreads();
+    for (int b = 0; b < batch; ++b) {
+      uint32_t most = 0;
+      for (int64_t j = threadIdx.x; j < v.dim; j += kMmaThreads) {
+        const uint32_t bits = __float_as_uint(load_value(x + b * ldx + j)) & 0x7fffffffu;
+        if (bits < 0x7f800000u && bits > most) most = bits;
+      }
+      most = __reduce_max_sync(0xffffffffu, most);
+      if (lane == 0 && most) atomicMax(&sh.largest[b], most);
+    }
+    __syncthreads();
+    if (threadIdx.x < kQ4SearchBatch) {
+      const uint32_t most = sh.largest[threadIdx.x];
+      int e = most ? 14 - (static_cast<int>(most >> 23) - 127) : 0;
+      if (e > 126) e = 126;
+      sh.factor[threadIdx.x] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+      sh.inverse[threadIdx.x] = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    }
+    __syncthreads();
   }
-  m = __reduce_min_sync(0xffffffffu, m);
-  if (lane == 0) minima[b * groups + g] = m;
+
+  // ---- a chunk of the vectors, as the matrix instruction takes them
+  const bool wide = ((reinterpret_cast<uintptr_t>(x) | (ldx * sizeof(T))) & 15) == 0;
+  auto stage_vectors = [&](int chunk) {
+    const int first = chunk * p.chunk_stages;
+    int len = p.stages - first;
+    if (len > p.chunk_stages) len = p.chunk_stages;
+    for (int item = threadIdx.x; item < len * 4 * kTiles * 32; item += kMmaThreads) {
+      const int l = item & 31, tile = (item >> 5) % kTiles, word = (item >> 5) / kTiles;
+      const int w = word & 3, column = l >> 2, q = l & 3;
+      int b, low;
+      if constexpr (kPacked) {
+        b = column & 3, low = column >> 2;
+      } else {
+        b = (tile % kOutTiles) * 8 + column, low = tile / kOutTiles;
+      }
+      int k = kStageCodes * (first + (word >> 2));
+      if constexpr (kGroups == 4) k += 32 * w + 8 * q;
+      else if constexpr (kGroups == 2) k += 64 * (w >> 1) + 16 * q + 8 * (w & 1);
+      else k += 32 * q + 8 * w;
+      float a[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a[e] = 0.0f;
+      if (b < batch && k < v.dim) {
+        const T* from = x + b * ldx + k;
+        if (wide && k + 8 <= v.dim) {
+          __align__(16) T h[8];
+#pragma unroll
+          for (int e = 0; e < static_cast<int>(sizeof(T)) / 2; ++e)
+            reinterpret_cast<uint4*>(h)[e] = reinterpret_cast<const uint4*>(from)[e];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) a[e] = load_value(h + e);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (k + e < v.dim) a[e] = load_value(from + e);
+        }
+      }
+      const float f = b < batch ? sh.factor[b] : 1.0f;
+      __half h[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float scaled = a[e] * f;
+        h[e] = __float2half_rn(scaled);
+        if (kParts == 2 && low) {
+          const float high = __half2float(h[e]);
+          h[e] = __float2half_rn(fabsf(high) <= 65504.0f ? scaled - high : 0.0f);
+        }
+      }
+      uint4 out;
+      out.x = __half_as_ushort(h[0]) | static_cast<uint32_t>(__half_as_ushort(h[4])) << 16;
+      out.y = __half_as_ushort(h[1]) | static_cast<uint32_t>(__half_as_ushort(h[5])) << 16;
+      out.z = __half_as_ushort(h[2]) | static_cast<uint32_t>(__half_as_ushort(h[6])) << 16;
+      out.w = __half_as_ushort(h[3]) | static_cast<uint32_t>(__half_as_ushort(h[7])) << 16;
+      vectors[item] = out;
+    }
+  };
+  stage_vectors(0);
+  __syncthreads();
+
+  // ---- scales and zero points of a stage: each lane has those of one group
+  // of its four rows (t % kGroups), and shares them with its neighbours
+  float scale[4], scale_next[4];
+  uint32_t zero[4], zero_next[4];
+  int32_t rows[4];
+  auto fetch_scales = [&](int slot_of_ring, int stage) {
+    const int j = kGroups * stage + (kGroups == 1 ? 0 : t % kGroups);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int32_t at = ring_rows[slot_of_ring * kTileRows4 + g + 8 * i];
+      scale_next[i] = 0.0f;
+      zero_next[i] = 8;
+      if (at >= 0 && j < v.groups) {
+        scale_next[i] = scale_of(v, at, j);
+        if (kZeros) zero_next[i] = v.zeros[static_cast<int64_t>(at) * v.groups + j] & 15u;
+      }
+    }
+  };
+
+  Cursor here = {0, 0, 0, 0};
+  here.enter(p, part);
+  __syncwarp();
+  fetch_scales(0, here.stage);
+  int ring_at = 0;  // the slot of the stage at hand
+  for (int iteration = 0; iteration < p.iterations; ++iteration) {
+    float total[2][kOutTiles][4] = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rows[i] = -1;
+    for (int chunk = 0; chunk < p.chunks; ++chunk) {
+      if (p.chunks > 1 && (iteration > 0 || chunk > 0)) {
+        __syncthreads();
+        stage_vectors(chunk);
+        __syncthreads();
+      }
+      while (here.iteration == iteration && here.chunk == chunk) {
+        copy_wait<kRing - 2>();
+        __syncwarp();
+        const int stage = here.stage;
+        const int ring_next = ring_at + 1 == kRing ? 0 : ring_at + 1;
+        send(ring_next + 1 == kRing ? 0 : ring_next + 1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          scale[i] = scale_next[i];
+          zero[i] = zero_next[i];
+          rows[i] = ring_rows[ring_at * kTileRows4 + g + 8 * i];
+        }
+        here.advance(p, part);
+        if (here.iteration < p.iterations) fetch_scales(ring_next, here.stage);
+
+        uint32_t words[4][4];
+        const uint8_t* codes = ring + ring_at * kStageBytes4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint8_t* c = codes + (g + 8 * i) * 64;
+          if constexpr (kGroups == 4) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              words[i][j] = *reinterpret_cast<const uint32_t*>(c + ((j ^ swizzle(g)) << 4) + 4 * t);
+          } else if constexpr (kGroups == 2) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint2 u = *reinterpret_cast<const uint2*>(
+                  c + (((2 * j + (t >> 1)) ^ swizzle(g)) << 4) + 8 * (t & 1));
+              words[i][2 * j] = u.x;
+              words[i][2 * j + 1] = u.y;
+            }
+          } else {
+            const uint4 u = *reinterpret_cast<const uint4*>(c + ((t ^ swizzle(g)) << 4));
+            words[i][0] = u.x, words[i][1] = u.y, words[i][2] = u.z, words[i][3] = u.w;
+          }
+        }
+        const uint4* vec = vectors + (stage - chunk * p.chunk_stages) * (4 * kTiles * 32) + lane;
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) {
+          float acc[2][kTiles][4] = {};
+          uint32_t one[4], sixteen[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t z = 8;
+            if (kZeros)
+              z = kGroups == 1 ? zero[i] : __shfl_sync(0xffffffffu, zero[i], (lane & 28) | j);
+            one[i] = 0x64006400u + z * 0x00010001u;      // 1024 + zero
+            sixteen[i] = 0xd400d400u + z * 0x00100010u;  // -(64 + zero)
+          }
+#pragma unroll
+          for (int w = j * kPerGroup; w < (j + 1) * kPerGroup; ++w) {
+            uint32_t a[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t u = words[i][w], far = u >> 8;
+              a[i][0] = sub2((u & 0x000f000fu) | 0x64006400u, one[i]);
+              a[i][1] = sixteenth2((u & 0x00f000f0u) | 0x64006400u, sixteen[i]);
+              a[i][2] = sub2((far & 0x000f000fu) | 0x64006400u, one[i]);
+              a[i][3] = sixteenth2((far & 0x00f000f0u) | 0x64006400u, sixteen[i]);
+            }
+#pragma unroll
+            for (int c = 0; c < kTiles; ++c) {
+              const uint4 b = vec[(w * kTiles + c) * 32];
+#pragma unroll
+              for (int m = 0; m < 2; ++m) {
+                mma_16816(acc[m][c], a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], b.x, b.y);
+                mma_16816(acc[m][c], a[2 * m][2], a[2 * m + 1][2], a[2 * m][3], a[2 * m + 1][3], b.z, b.w);
+              }
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float s =
+                kGroups == 1 ? scale[i] : __shfl_sync(0xffffffffu, scale[i], (lane & 28) | j);
+            const int m = i >> 1, h = 2 * (i & 1);
+#pragma unroll
+            for (int c = 0; c < kOutTiles; ++c)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float sum = acc[m][c][h + e];
+                if constexpr (!kPacked && kParts == 2) sum += acc[m][c + kOutTiles][h + e];
+                total[m][c][h + e] = fmaf(s, sum, total[m][c][h + e]);
+              }
+          }
+        }
+        ring_at = ring_next;
+      }
+    }
+    if constexpr (kPacked) {  // the low parts' columns are two lanes on
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          total[m][0][e] += __shfl_xor_sync(0xffffffffu, total[m][0][e], 2);
+    }
+    const int64_t first = tile_of(iteration) * kTileRows4;
+    if (p.split == 1) {
+#pragma unroll
+      for (int c = 0; c < kOutTiles; ++c)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int b = 8 * c + 2 * t + e;
+          const bool mine = b < batch && (!kPacked || t < 2);
+          uint32_t least = kNoKey;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int64_t at = first + g + 8 * i;
+            if (!mine || at >= r.count) continue;
+            float y = total[i >> 1][c][2 * (i & 1) + e] * sh.inverse[b];
+            if (rows[i] < 0) y = at < n ? __int_as_float(0x7fc00000) : 0.0f;
+            const float key = put(o, b, at, y, o.mode == kKeyL2 && rows[i] >= 0 ? v.norms[rows[i]] : 0.0f);
+            if (at < n) least = min(least, ordered(key));
+          }
+          if (o.minima) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1)
+              least = min(least, __shfl_xor_sync(0xffffffffu, least, d));
+            if (g == 0 && mine && first < r.count) o.minima[b * p.tiles + first / kTileRows4] = least;
+          }
+        }
+    } else {
+      float* mine = sums + warp * (kOutCols * kSumStride);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int c = 0; c < kOutTiles; ++c)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            mine[(8 * c + 2 * t + e) * kSumStride + g + 8 * i] = total[i >> 1][c][2 * (i & 1) + e];
+        if (part == 0 && t == 0) sh.tile_rows[slot][g + 8 * i] = rows[i];
+      }
+      __syncthreads();
+      // a warp to a tile and vector, a lane to a row
+      for (int item = warp; item < slots * batch; item += kMmaWarps) {
+        const int s = item / batch, b = item - s * batch;
+        const int64_t tile = (static_cast<int64_t>(iteration) * slots + s) * gridDim.x + blockIdx.x;
+        const int64_t at = tile * kTileRows4 + lane;
+        float y = 0.0f;
+        for (int q = 0; q < p.split; ++q)
+          y += sums[((s * p.split + q) * kOutCols + b) * kSumStride + lane];
+        y *= sh.inverse[b];
+        const int32_t from = sh.tile_rows[s][lane];
+        if (from < 0) y = at < n ? __int_as_float(0x7fc00000) : 0.0f;
+        uint32_t least = kNoKey;
+        if (at < r.count) {
+          const float key = put(o, b, at, y, o.mode == kKeyL2 && from >= 0 ? v.norms[from] : 0.0f);
+          if (at < n) least = ordered(key);
+        }
+        if (o.minima) {
+          least = __reduce_min_sync(0xffffffffu, least);
+          if (lane == 0 && tile < p.tiles) o.minima[b * p.tiles + tile] = least;
+        }
+      }
+      __syncthreads();
+    }
+  }
+  copy_wait<0>();
 }
+
+// ----------------------------------------------------------------- search
+constexpr int kGroupRows = kTileRows4;  // rows whose smallest key is kept
+constexpr int kSelectThreads = 1024;
+constexpr int kMoreCandidates = 16;  // scored again beyond the k asked for
+constexpr int kMaxCandidates = KNN_MAX_K + kMoreCandidates;
+constexpr int kGroupCap = 1024;
+constexpr int kCandCap = 4096;
 
 struct SelectSmem {
   uint64_t cand[kCandCap];
@@ -553,19 +962,82 @@ unsigned row_grid(int64_t rows) {
       std::max<int64_t>(1, std::min<int64_t>((rows + kWarps - 1) / kWarps, 148 * 8)));
 }
 
-template <class T>
-cudaError_t products(const Q4View& v, const Q4Range& r, const void* x, int64_t batch, int64_t ldx,
-                     const Q4Out& o, cudaStream_t stream) {
-  store_count_launches(1);
-  return launch_after(products_kernel<T>, row_grid(r.count), kThreads, 0, stream, v, r,
-                      static_cast<const T*>(x), batch, ldx, o);
+// Shared memory of a block beside the vectors.
+int64_t mma_fixed_bytes(int split, int out_cols) {
+  return kMmaWarps * kRing * (kStageBytes4 + 4 * kTileRows4) +
+         (split > 1 ? kMmaWarps * out_cols * kSumStride * 4 : 0);
 }
 
-cudaError_t products_any(const Q4View& v, const Q4Range& r, const void* x, int dtype,
-                         int64_t batch, int64_t ldx, const Q4Out& o, cudaStream_t stream) {
-  if (dtype == KNN_DTYPE_F32) return products<float>(v, r, x, batch, ldx, o, stream);
-  if (dtype == KNN_DTYPE_F16) return products<__half>(v, r, x, batch, ldx, o, stream);
-  return products<__nv_bfloat16>(v, r, x, batch, ldx, o, stream);
+// Warps that share a tile: the number with the least time of a block, in
+// stages.  A tile that is shared costs about a stage more for adding up.
+int mma_split(int64_t tiles, int stages, int sms) {
+  int best = 1;
+  double least = 0;
+  for (int split = 1; split <= kMmaWarps && split <= stages; split *= 2) {
+    const int64_t at_once = static_cast<int64_t>(sms) * (kMmaWarps / split);
+    const double time = static_cast<double>((tiles + at_once - 1) / at_once) *
+                        ((stages + split - 1) / split + (split > 1 ? 1.0 : 0.25));
+    if (split == 1 || time < least) least = time, best = split;
+  }
+  return best;
+}
+
+template <class T, int kTiles, int kParts, int kGroups, bool kZeros>
+cudaError_t products(const Q4View& v, const Q4Range& r, const T* x, int batch, int64_t ldx,
+                     const Q4Out& o, cudaStream_t stream) {
+  constexpr int kOutCols = kTiles == 1 ? 8 : 8 * kTiles / kParts;
+  constexpr int64_t kMost = 232448 - sizeof(MmaShared) - 64;
+  auto kernel = products_kernel<T, kTiles, kParts, kGroups, kZeros>;
+  const int sms = store_sm_count();
+  MmaPlan p;
+  p.tiles = (r.count + kTileRows4 - 1) / kTileRows4;
+  p.stages = static_cast<int32_t>((v.dim + kStageCodes - 1) / kStageCodes);
+  p.split = mma_split(p.tiles, p.stages, sms);
+  const int64_t room = (kMost - mma_fixed_bytes(2, kOutCols)) / (4 * kTiles * 512);
+  p.chunk_stages = static_cast<int32_t>(std::min<int64_t>(p.stages, room));
+  while (p.split > p.chunk_stages) p.split /= 2;  // every warp has a stage of every full chunk
+  p.chunks = (p.stages + p.chunk_stages - 1) / p.chunk_stages;
+  const int64_t grid = std::min<int64_t>(p.tiles, sms);
+  const int64_t slots = kMmaWarps / p.split;
+  p.iterations = static_cast<int32_t>((p.tiles + grid * slots - 1) / (grid * slots));
+  const size_t smem = mma_fixed_bytes(p.split, kOutCols) + p.chunk_stages * (4 * kTiles * 512);
+  static std::atomic<uint64_t> allowed{0};
+  if (cudaError_t e = allow_smem(kernel, static_cast<int>(kMost), &allowed)) return e;
+  store_count_launches(1);
+  return launch_after(kernel, static_cast<unsigned>(grid), kMmaThreads, smem, stream, v, r, x,
+                      batch, ldx, o, p);
+}
+
+template <class T, int kTiles, int kParts>
+cudaError_t products_of(const Q4View& v, const Q4Range& r, const T* x, int batch, int64_t ldx,
+                        const Q4Out& o, cudaStream_t stream) {
+  if (v.group == 32)
+    return v.zeros ? products<T, kTiles, kParts, 4, true>(v, r, x, batch, ldx, o, stream)
+                   : products<T, kTiles, kParts, 4, false>(v, r, x, batch, ldx, o, stream);
+  if (v.group == 64)
+    return v.zeros ? products<T, kTiles, kParts, 2, true>(v, r, x, batch, ldx, o, stream)
+                   : products<T, kTiles, kParts, 2, false>(v, r, x, batch, ldx, o, stream);
+  return v.zeros ? products<T, kTiles, kParts, 1, true>(v, r, x, batch, ldx, o, stream)
+                 : products<T, kTiles, kParts, 1, false>(v, r, x, batch, ldx, o, stream);
+}
+
+// Up to kQ4SearchBatch vectors in one pass over the rows.
+cudaError_t products_any(const Q4View& v, const Q4Range& r, const void* x, int dtype, int batch,
+                         int64_t ldx, const Q4Out& o, cudaStream_t stream) {
+  if (dtype == KNN_DTYPE_F32) {
+    const float* f = static_cast<const float*>(x);
+    if (batch <= 4) return products_of<float, 1, 2>(v, r, f, batch, ldx, o, stream);
+    if (batch <= 8) return products_of<float, 2, 2>(v, r, f, batch, ldx, o, stream);
+    return products_of<float, 4, 2>(v, r, f, batch, ldx, o, stream);
+  }
+  if (dtype == KNN_DTYPE_F16) {
+    const __half* f = static_cast<const __half*>(x);
+    if (batch <= 8) return products_of<__half, 1, 1>(v, r, f, batch, ldx, o, stream);
+    return products_of<__half, 2, 1>(v, r, f, batch, ldx, o, stream);
+  }
+  const __nv_bfloat16* f = static_cast<const __nv_bfloat16*>(x);
+  if (batch <= 8) return products_of<__nv_bfloat16, 1, 1>(v, r, f, batch, ldx, o, stream);
+  return products_of<__nv_bfloat16, 2, 1>(v, r, f, batch, ldx, o, stream);
 }
 
 int64_t group_count(int64_t count) { return (count + kGroupRows - 1) / kGroupRows; }
@@ -574,11 +1046,8 @@ template <class T>
 cudaError_t select(const Q4View& v, const Q4Range& r, const void* x, int64_t batch, int64_t ldx,
                    const float* keys, int64_t ld, const uint32_t* minima, int k, int mode,
                    int64_t* neighbors, float* distances, cudaStream_t stream) {
-  // above 48 KB only by leave, once per device and kernel
-  cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(select_kernel<T>),
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       sizeof(SelectSmem));
-  if (e != cudaSuccess) return e;
+  static std::atomic<uint64_t> allowed{0};
+  if (cudaError_t e = allow_smem(select_kernel<T>, sizeof(SelectSmem), &allowed)) return e;
   store_count_launches(1);
   return launch_after(select_kernel<T>, static_cast<unsigned>(batch), kSelectThreads,
                       sizeof(SelectSmem), stream, v, r, static_cast<const T*>(x), ldx, keys, ld,
@@ -613,7 +1082,15 @@ cudaError_t launch_q4_read(const Q4View& v, const Q4List& l, float* out, int64_t
 cudaError_t launch_q4_products(const Q4View& v, const Q4Range& r, const void* x, int dtype,
                                int64_t batch, int64_t ldx, void* out, int out_dtype, int64_t ldo,
                                cudaStream_t stream) {
-  return products_any(v, r, x, dtype, batch, ldx, Q4Out{out, out_dtype, ldo, kStore}, stream);
+  const int64_t size = dtype == KNN_DTYPE_F32 ? 4 : 2, out_size = out_dtype == KNN_DTYPE_F32 ? 4 : 2;
+  for (int64_t b = 0; b < batch; b += kQ4SearchBatch) {
+    const Q4Out o = {static_cast<char*>(out) + b * ldo * out_size, out_dtype, ldo, kStore, nullptr};
+    if (cudaError_t e = products_any(
+            v, r, static_cast<const char*>(x) + b * ldx * size, dtype,
+            static_cast<int>(std::min<int64_t>(kQ4SearchBatch, batch - b)), ldx, o, stream))
+      return e;
+  }
+  return cudaSuccess;
 }
 
 int64_t q4_search_bytes(int64_t count) {
@@ -632,18 +1109,8 @@ cudaError_t launch_q4_search(const Q4View& v, const Q4Range& r, const void* x, i
     const int64_t m = std::min<int64_t>(kQ4SearchBatch, batch - b);
     const void* q = static_cast<const char*>(x) + b * ldx * size;
     if (r.count > 0) {
-      if (cudaError_t e = products_any(v, r, q, dtype, m, ldx,
-                                       Q4Out{keys, KNN_DTYPE_F32, ld, mode}, stream))
-        return e;
-      store_count_launches(1);
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3(static_cast<unsigned>((groups + kWarps - 1) / kWarps),
-                         static_cast<unsigned>(m));
-      cfg.blockDim = dim3(kThreads);
-      cfg.stream = stream;
-      if (cudaError_t e = cudaLaunchKernelEx(&cfg, group_min_kernel, r,
-                                             static_cast<const float*>(keys), ld, minima, groups))
-        return e;
+      const Q4Out o = {keys, KNN_DTYPE_F32, ld, mode, minima};
+      if (cudaError_t e = products_any(v, r, q, dtype, static_cast<int>(m), ldx, o, stream)) return e;
     }
     cudaError_t e;
     if (dtype == KNN_DTYPE_F32)

@@ -2,6 +2,7 @@
 // 4 bits (knn_pages.cu, knn_q4.cu, knn_store_capi.cu).
 #pragma once
 
+#include <atomic>
 #include <cstdint>
 #include <cuda_runtime.h>
 
@@ -52,6 +53,32 @@ cudaError_t launch_after(void (*kernel)(P...), unsigned grid, unsigned block, si
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+// Leave for a kernel to use `bytes` of dynamic shared memory on the current
+// device, asked for once a device (`allowed` has a bit for each of the first 64).
+template <class K>
+cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>* allowed) {
+  int device = 0;
+  if (cudaError_t e = cudaGetDevice(&device)) return e;
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (allowed->load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) allowed->fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
+// Multiprocessors of the current device.
+inline int store_sm_count() {
+  static std::atomic<int> counts[64];
+  int device = 0, sms = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return 148;
+  if (device < 64 && (sms = counts[device].load(std::memory_order_relaxed)) > 0) return sms;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms < 1)
+    return 148;
+  if (device < 64) counts[device].store(sms, std::memory_order_relaxed);
+  return sms;
 }
 
 __device__ __forceinline__ void wait_for_stream() {
