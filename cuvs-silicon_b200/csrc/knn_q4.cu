@@ -335,13 +335,17 @@ struct MmaPlan {
   int32_t split;  // warps that share a tile
 };
 
+// Dynamic shared memory: ring[warp][slot][kStageBytes4], then scales[warp][2]
+// [groups of a stage][32 rows] and zero points likewise, then (split > 1)
+// sums[warp][column][kSumStride], then the vectors.
 struct MmaShared {
-  // ring[warp][slot][kStageBytes4], then rows[warp][slot][32], then sums
-  // (where split > 1) [warp][columns][kSumStride], then vectors
   uint32_t largest[kQ4SearchBatch];
   float factor[kQ4SearchBatch], inverse[kQ4SearchBatch];
-  int32_t tile_rows[kMmaWarps][kTileRows4];
+  // rows of the tiles that a warp is at, by iteration: it copies ahead by at
+  // most kRing - 1 stages, so by as many tiles
+  int32_t rows[kMmaWarps][4][kTileRows4];
 };
+static_assert(kRing - 1 < 4, "the tiles at hand have places of their own");
 
 __device__ __forceinline__ void copy_ahead(void* to, const void* from, bool valid) {
   const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(to));
@@ -358,15 +362,22 @@ __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
 }
 
+// d = a b + c
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                          uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                                          uint32_t a3, uint32_t b0, uint32_t b1, float c0,
+                                          float c1, float c2, float c3) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
+// (a & b) | c in one instruction
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
 __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
   const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
@@ -383,31 +394,20 @@ __device__ __forceinline__ uint32_t sixteenth2(uint32_t a, uint32_t c) {
 // bytes a lane) meet no bank twice.
 __device__ __forceinline__ int swizzle(int row) { return (row & 2) | ((row >> 2) & 1); }
 
-// A warp's place in its work: tile after tile, in each chunk after chunk, in
-// each the stages of its part.
-struct Cursor {
-  int32_t iteration, chunk, stage, end;
-  __device__ __forceinline__ void enter(const MmaPlan& p, int part) {
-    const int first = chunk * p.chunk_stages;
-    int len = p.stages - first;
-    if (len > p.chunk_stages) len = p.chunk_stages;
-    stage = first + part * len / p.split;
-    end = first + (part + 1) * len / p.split;
-  }
-  // To the next stage; true where a new tile begins.
-  __device__ __forceinline__ bool advance(const MmaPlan& p, int part) {
-    bool fresh = false;
-    ++stage;
-    while (stage >= end && iteration < p.iterations) {
-      if (++chunk == p.chunks) {
-        chunk = 0;
-        ++iteration;
-        fresh = true;
-      }
-      enter(p, part);
-    }
-    return fresh;
-  }
+// The stages of a chunk that fall to a warp.
+__device__ __forceinline__ void part_of(const MmaPlan& p, int chunk, int part, int* first, int* end) {
+  const int start = chunk * p.chunk_stages;
+  int len = p.stages - start;
+  if (len > p.chunk_stages) len = p.chunk_stages;
+  *first = start + part * len / p.split;
+  *end = start + (part + 1) * len / p.split;
+}
+
+// The scales and zero points of a stage's groups in one row, as they are held.
+template <int kGroups>
+struct HeldScales {
+  uint32_t s[(kGroups + 1) / 2];
+  uint32_t z;
 };
 
 // kCols: columns of the matrix instruction in tiles of 8 (kTiles of them);
@@ -426,9 +426,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
   uint8_t* ring = raw + warp * (kRing * kStageBytes4);
-  int32_t* ring_rows = reinterpret_cast<int32_t*>(raw + kMmaWarps * kRing * kStageBytes4) +
-                       warp * (kRing * kTileRows4);
-  float* sums = reinterpret_cast<float*>(raw + kMmaWarps * kRing * (kStageBytes4 + 4 * kTileRows4));
+  constexpr int kScales = kGroups * kTileRows4;  // words of a stage's scales
+  uint32_t* scales = reinterpret_cast<uint32_t*>(raw + kMmaWarps * kRing * kStageBytes4) +
+                     warp * (2 * kScales * (kZeros ? 2 : 1));
+  float* sums = reinterpret_cast<float*>(raw + kMmaWarps * kRing * kStageBytes4 +
+                                         kMmaWarps * 2 * kScales * (kZeros ? 2 : 1) * 4);
   uint4* vectors = reinterpret_cast<uint4*>(
       reinterpret_cast<uint8_t*>(sums) +
       (p.split > 1 ? kMmaWarps * kOutCols * kSumStride * sizeof(float) : 0));
@@ -448,32 +450,91 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     return i < n ? static_cast<int32_t>(v.places.at(r.seq, i)) : -1;
   };
 
-  // ---- copying codes ahead
-  Cursor ahead = {0, 0, 0, 0};
-  ahead.enter(p, part);
-  int32_t row = row_of(0), row_next = row_of(1);
-  auto send = [&](int slot_of_ring) {
-    if (ahead.iteration < p.iterations) {
-      uint8_t* to = ring + slot_of_ring * kStageBytes4;
-      const int c = 4 * ahead.stage + t;
+  // ---- copying codes ahead, and the scales with them.  Lane (g, t) copies 16
+  // bytes of rows g, g + 8, g + 16 and g + 24, and holds the scales of row
+  // g + 8 t.  A row that does not exist is read as the tile's first that does;
+  // what comes of it is replaced in the end.  (Reading row 0 instead made
+  // every warp that had run out of rows ask for the same few lines: a million
+  // rows took 208 us instead of 103.)  A tile without rows copies nothing.
+  int next_iteration = 0, next_chunk = 0, next_stage, next_end;
+  part_of(p, 0, part, &next_stage, &next_end);
+  int32_t row_after = row_of(0);
+  const uint8_t* from[4];
+  int64_t scales_at = 0;
+  bool some = false;  // the tile has rows
+  const bool together = v.groups % kGroups == 0 &&
+                        reinterpret_cast<uintptr_t>(v.scales) % (2 * kGroups) == 0 &&
+                        (!kZeros || reinterpret_cast<uintptr_t>(v.zeros) % kGroups == 0);
+  auto enter_tile = [&]() {
+    const int32_t row = row_after;
+    sh.rows[warp][next_iteration & 3][lane] = row;
+    row_after = row_of(next_iteration + 1);
+    const uint32_t exist = __ballot_sync(0xffffffffu, row >= 0);
+    some = exist != 0;
+    const int32_t first = __shfl_sync(0xffffffffu, row, some ? __ffs(exist) - 1 : 0);
+    const int32_t read = row >= 0 ? row : some ? first : 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int32_t at = __shfl_sync(0xffffffffu, row, g + 8 * i);
-        const bool valid = at >= 0 && 16 * c < v.width;
-        const uint8_t* from = v.codes + (valid ? static_cast<int64_t>(at) * v.width + 16 * c : 0);
-        copy_ahead(to + (g + 8 * i) * 64 + ((t ^ swizzle(g)) << 4), from, valid);
+    for (int i = 0; i < 4; ++i)
+      from[i] = v.codes + static_cast<int64_t>(__shfl_sync(0xffffffffu, read, g + 8 * i)) * v.width + 16 * t;
+    scales_at = static_cast<int64_t>(__shfl_sync(0xffffffffu, read, g + 8 * t)) * v.groups;
+  };
+  enter_tile();
+  const int quarters = v.width >> 4;  // 16-byte pieces of a row
+  const int to_lane = g * 64 + ((t ^ swizzle(g)) << 4);
+  HeldScales<kGroups> held;
+  auto send = [&](uint8_t* to) {
+    if (next_iteration < p.iterations) {
+      const bool valid = some && 4 * next_stage + t < quarters;
+      const uint32_t ahead = valid ? 64u * next_stage : 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) copy_ahead(to + to_lane + i * 512, from[i] + ahead, valid);
+      const int64_t j = scales_at + kGroups * next_stage;
+      held = {};
+      if (!some) {
+      } else if (kGroups == 1 || together) {
+        if constexpr (kGroups == 1) held.s[0] = v.scales[j];
+        if constexpr (kGroups == 2) held.s[0] = *reinterpret_cast<const uint32_t*>(v.scales + j);
+        if constexpr (kGroups == 4) {
+          const uint2 u = *reinterpret_cast<const uint2*>(v.scales + j);
+          held.s[0] = u.x, held.s[kGroups / 4] = u.y;
+        }
+        if constexpr (kZeros && kGroups == 1) held.z = v.zeros[j];
+        if constexpr (kZeros && kGroups == 2) held.z = *reinterpret_cast<const uint16_t*>(v.zeros + j);
+        if constexpr (kZeros && kGroups == 4) held.z = *reinterpret_cast<const uint32_t*>(v.zeros + j);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kGroups; ++e)
+          if (kGroups * next_stage + e < v.groups) {
+            held.s[e >> 1] |= static_cast<uint32_t>(v.scales[j + e]) << (16 * (e & 1));
+            if (kZeros) held.z |= static_cast<uint32_t>(v.zeros[j + e]) << (8 * e);
+          }
       }
-      ring_rows[slot_of_ring * kTileRows4 + lane] = row;
-      if (ahead.advance(p, part)) {
-        row = row_next;
-        row_next = row_of(ahead.iteration + 1);
+      if (++next_stage == next_end) {
+        do {
+          if (++next_chunk == p.chunks) {
+            next_chunk = 0;
+            if (++next_iteration < p.iterations) enter_tile();
+          }
+          part_of(p, next_chunk, part, &next_stage, &next_end);
+        } while (next_stage == next_end);
       }
     }
     copy_close();
   };
+  // Puts the scales that came with the last stage sent where every lane of the
+  // warp finds those of its four rows side by side, as fp32, and 1024 + zero
+  // point, twice, in fp16.
+  auto put_scales = [&](uint32_t* to) {
 #pragma unroll
-  for (int j = 0; j < kRing - 1; ++j) send(j);
-
+    for (int j = 0; j < kGroups; ++j) {
+      const uint32_t bits = (held.s[j >> 1] >> (16 * (j & 1))) & 0xffffu;
+      const float as_half = __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+      to[j * kTileRows4 + lane] = v.scale_bf16 ? bits << 16 : __float_as_uint(as_half);
+      if (kZeros)
+        to[2 * kScales + j * kTileRows4 + lane] =
+            0x64006400u + ((held.z >> (8 * j)) & 15u) * 0x00010001u;
+    }
+  };
   // ---- the vectors' scales
   if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
     if (threadIdx.x < kQ4SearchBatch) sh.factor[threadIdx.x] = sh.inverse[threadIdx.x] = 1.0f;
@@ -557,62 +618,42 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     }
   };
   stage_vectors(0);
+  send(ring);
+  put_scales(scales);
+  send(ring + kStageBytes4);
+  static_assert(kRing == 3, "the stage at hand, the next, and the one being sent");
+
   __syncthreads();
 
-  // ---- scales and zero points of a stage: each lane has those of one group
-  // of its four rows (t % kGroups), and shares them with its neighbours
-  float scale[4], scale_next[4];
-  uint32_t zero[4], zero_next[4];
-  int32_t rows[4];
-  auto fetch_scales = [&](int slot_of_ring, int stage) {
-    const int j = kGroups * stage + (kGroups == 1 ? 0 : t % kGroups);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int32_t at = ring_rows[slot_of_ring * kTileRows4 + g + 8 * i];
-      scale_next[i] = 0.0f;
-      zero_next[i] = 8;
-      if (at >= 0 && j < v.groups) {
-        scale_next[i] = scale_of(v, at, j);
-        if (kZeros) zero_next[i] = v.zeros[static_cast<int64_t>(at) * v.groups + j] & 15u;
-      }
-    }
-  };
-
-  Cursor here = {0, 0, 0, 0};
-  here.enter(p, part);
-  __syncwarp();
-  fetch_scales(0, here.stage);
-  int ring_at = 0;  // the slot of the stage at hand
+  uint32_t ring_at = 0, ring_free = (kRing - 1) * kStageBytes4;  // bytes into the ring
+  uint32_t scales_now = 0;                                       // words into the scales
   for (int iteration = 0; iteration < p.iterations; ++iteration) {
     float total[2][kOutTiles][4] = {};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) rows[i] = -1;
     for (int chunk = 0; chunk < p.chunks; ++chunk) {
       if (p.chunks > 1 && (iteration > 0 || chunk > 0)) {
         __syncthreads();
         stage_vectors(chunk);
         __syncthreads();
       }
-      while (here.iteration == iteration && here.chunk == chunk) {
+      int stage, end;
+      part_of(p, chunk, part, &stage, &end);
+      const uint4* vec = vectors + (stage - chunk * p.chunk_stages) * (4 * kTiles * 32) + lane;
+#pragma unroll 1
+      for (; stage < end; ++stage, vec += 4 * kTiles * 32) {
         copy_wait<kRing - 2>();
         __syncwarp();
-        const int stage = here.stage;
-        const int ring_next = ring_at + 1 == kRing ? 0 : ring_at + 1;
-        send(ring_next + 1 == kRing ? 0 : ring_next + 1);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          scale[i] = scale_next[i];
-          zero[i] = zero_next[i];
-          rows[i] = ring_rows[ring_at * kTileRows4 + g + 8 * i];
-        }
-        here.advance(p, part);
-        if (here.iteration < p.iterations) fetch_scales(ring_next, here.stage);
+        const uint32_t* scale_row = scales + scales_now + 4 * g;
+        scales_now ^= kScales;
+        put_scales(scales + scales_now);  // of the next stage
+        send(ring + ring_free);
+        const uint8_t* codes = ring + ring_at + g * 64;
+        ring_free = ring_at;
+        ring_at = ring_at == (kRing - 1) * kStageBytes4 ? 0 : ring_at + kStageBytes4;
 
         uint32_t words[4][4];
-        const uint8_t* codes = ring + ring_at * kStageBytes4;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint8_t* c = codes + (g + 8 * i) * 64;
+          const uint8_t* c = codes + i * 512;
           if constexpr (kGroups == 4) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -630,44 +671,47 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
             words[i][0] = u.x, words[i][1] = u.y, words[i][2] = u.z, words[i][3] = u.w;
           }
         }
-        const uint4* vec = vectors + (stage - chunk * p.chunk_stages) * (4 * kTiles * 32) + lane;
 #pragma unroll
         for (int j = 0; j < kGroups; ++j) {
-          float acc[2][kTiles][4] = {};
+          float acc[2][kTiles][4];
           uint32_t one[4], sixteen[4];
+          const float4 s4 = *reinterpret_cast<const float4*>(scale_row + j * kTileRows4);
+          const float scale[4] = {s4.x, s4.y, s4.z, s4.w};
+          uint4 z4 = make_uint4(0x64086408u, 0x64086408u, 0x64086408u, 0x64086408u);
+          if (kZeros) z4 = *reinterpret_cast<const uint4*>(scale_row + 2 * kScales + j * kTileRows4);
+          one[0] = z4.x, one[1] = z4.y, one[2] = z4.z, one[3] = z4.w;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t z = 8;
-            if (kZeros)
-              z = kGroups == 1 ? zero[i] : __shfl_sync(0xffffffffu, zero[i], (lane & 28) | j);
-            one[i] = 0x64006400u + z * 0x00010001u;      // 1024 + zero
-            sixteen[i] = 0xd400d400u + z * 0x00100010u;  // -(64 + zero)
-          }
+          for (int i = 0; i < 4; ++i) sixteen[i] = ((one[i] & 0x000f000fu) << 4) | 0xd400d400u;  // -(64 + zero)
 #pragma unroll
           for (int w = j * kPerGroup; w < (j + 1) * kPerGroup; ++w) {
             uint32_t a[4][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const uint32_t u = words[i][w], far = u >> 8;
-              a[i][0] = sub2((u & 0x000f000fu) | 0x64006400u, one[i]);
-              a[i][1] = sixteenth2((u & 0x00f000f0u) | 0x64006400u, sixteen[i]);
-              a[i][2] = sub2((far & 0x000f000fu) | 0x64006400u, one[i]);
-              a[i][3] = sixteenth2((far & 0x00f000f0u) | 0x64006400u, sixteen[i]);
+              a[i][0] = sub2(and_or(u, 0x000f000fu, 0x64006400u), one[i]);
+              a[i][1] = sixteenth2(and_or(u, 0x00f000f0u, 0x64006400u), sixteen[i]);
+              a[i][2] = sub2(and_or(far, 0x000f000fu, 0x64006400u), one[i]);
+              a[i][3] = sixteenth2(and_or(far, 0x00f000f0u, 0x64006400u), sixteen[i]);
             }
 #pragma unroll
             for (int c = 0; c < kTiles; ++c) {
               const uint4 b = vec[(w * kTiles + c) * 32];
 #pragma unroll
               for (int m = 0; m < 2; ++m) {
-                mma_16816(acc[m][c], a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], b.x, b.y);
-                mma_16816(acc[m][c], a[2 * m][2], a[2 * m + 1][2], a[2 * m][3], a[2 * m + 1][3], b.z, b.w);
+                float(&d)[4] = acc[m][c];
+                if (w == j * kPerGroup)
+                  mma_16816(d, a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], b.x, b.y,
+                            0.0f, 0.0f, 0.0f, 0.0f);
+                else
+                  mma_16816(d, a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], b.x, b.y,
+                            d[0], d[1], d[2], d[3]);
+                mma_16816(d, a[2 * m][2], a[2 * m + 1][2], a[2 * m][3], a[2 * m + 1][3], b.z, b.w,
+                          d[0], d[1], d[2], d[3]);
               }
             }
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float s =
-                kGroups == 1 ? scale[i] : __shfl_sync(0xffffffffu, scale[i], (lane & 28) | j);
             const int m = i >> 1, h = 2 * (i & 1);
 #pragma unroll
             for (int c = 0; c < kOutTiles; ++c)
@@ -675,13 +719,15 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
               for (int e = 0; e < 2; ++e) {
                 float sum = acc[m][c][h + e];
                 if constexpr (!kPacked && kParts == 2) sum += acc[m][c + kOutTiles][h + e];
-                total[m][c][h + e] = fmaf(s, sum, total[m][c][h + e]);
+                total[m][c][h + e] = fmaf(scale[i], sum, total[m][c][h + e]);
               }
           }
         }
-        ring_at = ring_next;
       }
     }
+    int32_t rows[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rows[i] = sh.rows[warp][iteration & 3][g + 8 * i];
     if constexpr (kPacked) {  // the low parts' columns are two lanes on
 #pragma unroll
       for (int m = 0; m < 2; ++m)
@@ -723,7 +769,6 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
             mine[(8 * c + 2 * t + e) * kSumStride + g + 8 * i] = total[i >> 1][c][2 * (i & 1) + e];
-        if (part == 0 && t == 0) sh.tile_rows[slot][g + 8 * i] = rows[i];
       }
       __syncthreads();
       // a warp to a tile and vector, a lane to a row
@@ -735,11 +780,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         for (int q = 0; q < p.split; ++q)
           y += sums[((s * p.split + q) * kOutCols + b) * kSumStride + lane];
         y *= sh.inverse[b];
-        const int32_t from = sh.tile_rows[s][lane];
-        if (from < 0) y = at < n ? __int_as_float(0x7fc00000) : 0.0f;
+        const int32_t at_row = sh.rows[s * p.split][iteration & 3][lane];
+        if (at_row < 0) y = at < n ? __int_as_float(0x7fc00000) : 0.0f;
         uint32_t least = kNoKey;
         if (at < r.count) {
-          const float key = put(o, b, at, y, o.mode == kKeyL2 && from >= 0 ? v.norms[from] : 0.0f);
+          const float key = put(o, b, at, y, o.mode == kKeyL2 && at_row >= 0 ? v.norms[at_row] : 0.0f);
           if (at < n) least = ordered(key);
         }
         if (o.minima) {
@@ -963,8 +1008,9 @@ unsigned row_grid(int64_t rows) {
 }
 
 // Shared memory of a block beside the vectors.
-int64_t mma_fixed_bytes(int split, int out_cols) {
-  return kMmaWarps * kRing * (kStageBytes4 + 4 * kTileRows4) +
+int64_t mma_fixed_bytes(int split, int out_cols, int groups, bool zeros) {
+  return kMmaWarps * kRing * kStageBytes4 +
+         kMmaWarps * 2 * groups * kTileRows4 * 4 * (zeros ? 2 : 1) +
          (split > 1 ? kMmaWarps * out_cols * kSumStride * 4 : 0);
 }
 
@@ -993,14 +1039,14 @@ cudaError_t products(const Q4View& v, const Q4Range& r, const T* x, int batch, i
   p.tiles = (r.count + kTileRows4 - 1) / kTileRows4;
   p.stages = static_cast<int32_t>((v.dim + kStageCodes - 1) / kStageCodes);
   p.split = mma_split(p.tiles, p.stages, sms);
-  const int64_t room = (kMost - mma_fixed_bytes(2, kOutCols)) / (4 * kTiles * 512);
+  const int64_t room = (kMost - mma_fixed_bytes(2, kOutCols, kGroups, kZeros)) / (4 * kTiles * 512);
   p.chunk_stages = static_cast<int32_t>(std::min<int64_t>(p.stages, room));
   while (p.split > p.chunk_stages) p.split /= 2;  // every warp has a stage of every full chunk
   p.chunks = (p.stages + p.chunk_stages - 1) / p.chunk_stages;
   const int64_t grid = std::min<int64_t>(p.tiles, sms);
   const int64_t slots = kMmaWarps / p.split;
   p.iterations = static_cast<int32_t>((p.tiles + grid * slots - 1) / (grid * slots));
-  const size_t smem = mma_fixed_bytes(p.split, kOutCols) + p.chunk_stages * (4 * kTiles * 512);
+  const size_t smem = mma_fixed_bytes(p.split, kOutCols, kGroups, kZeros) + p.chunk_stages * (4 * kTiles * 512);
   static std::atomic<uint64_t> allowed{0};
   if (cudaError_t e = allow_smem(kernel, static_cast<int>(kMost), &allowed)) return e;
   store_count_launches(1);
