@@ -306,7 +306,7 @@ __device__ __forceinline__ float put(const Q4Out& o, int64_t b, int64_t i, float
 // after the group's scaling): x = high + low is off by at most 2^-24 |x| +
 // 2^-40 max|x|, a bf16 one by 2^-40 max|x| at the very most.
 //
-// A warp takes tiles of 32 rows and runs down their codes in stages of 128,
+// A warp takes tiles of 32 rows and runs down their codes in stages of 256,
 // which it copies ahead into a ring of its own in shared memory (cp.async, no
 // barrier between warps); the ring also hands the codes of a group to the
 // lanes that the matrix instruction wants them in.  The order of the values
@@ -320,32 +320,31 @@ __device__ __forceinline__ float put(const Q4Out& o, int64_t b, int64_t i, float
 // up through shared memory, in order.
 constexpr int kMmaWarps = 16;
 constexpr int kMmaThreads = 32 * kMmaWarps;
-constexpr int kTileRows4 = 32;  // rows of a tile
-constexpr int kStageCodes = 128;
+constexpr int kTileRows4 = 32;    // rows of a tile
+constexpr int kStageCodes = 256;  // codes of a row in a stage: two halves
 constexpr int kStageBytes4 = kTileRows4 * kStageCodes / 2;
-constexpr int kRing = 3;
-constexpr int kSumStride = 36;  // floats from column to column of a tile's sums: no bank twice
+constexpr int kRing = 2;          // the stage at hand and the next
+constexpr int kSumStride = 36;    // floats from column to column of a tile's sums: no bank twice
 
 struct MmaPlan {
   int64_t tiles;
-  int32_t iterations;    // tiles that a warp's slot goes through
-  int32_t stages;        // of 128 codes in a row
+  int32_t iterations;    // tiles that a warp's slot goes through, at most
+  int32_t stages;        // of 256 codes in a row
   int32_t chunk_stages;  // stages whose share of the vectors fits in shared memory
   int32_t chunks;
   int32_t split;  // warps that share a tile
 };
 
-// Dynamic shared memory: ring[warp][slot][kStageBytes4], then scales[warp][2]
-// [groups of a stage][32 rows] and zero points likewise, then (split > 1)
-// sums[warp][column][kSumStride], then the vectors.
+// Dynamic shared memory: ring[warp][kRing][kStageBytes4], then scales[warp][2]
+// [groups of a stage][32 rows], then (split > 1) sums[warp][vector]
+// [kSumStride], then the vectors.
 struct MmaShared {
   uint32_t largest[kQ4SearchBatch];
   float factor[kQ4SearchBatch], inverse[kQ4SearchBatch];
-  // rows of the tiles that a warp is at, by iteration: it copies ahead by at
-  // most kRing - 1 stages, so by as many tiles
+  // rows of the tiles that a warp is at, by iteration: it copies ahead by up
+  // to two stages, so by as many tiles
   int32_t rows[kMmaWarps][4][kTileRows4];
 };
-static_assert(kRing - 1 < 4, "the tiles at hand have places of their own");
 
 __device__ __forceinline__ void copy_ahead(void* to, const void* from, bool valid) {
   const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(to));
@@ -389,10 +388,12 @@ __device__ __forceinline__ uint32_t sixteenth2(uint32_t a, uint32_t c) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// Which 16 bytes of a row's 64 in a stage lie where: rows 0 .. 7 put them at
-// chunk ^ swizzle(row), so that the three ways below to read them (4, 8 or 16
-// bytes a lane) meet no bank twice.
-__device__ __forceinline__ int swizzle(int row) { return (row & 2) | ((row >> 2) & 1); }
+// Which 16 bytes of a row's 128 in a stage lie where: rows 0 .. 7 put them at
+// piece ^ swizzle(row), the row's bits in reverse, so that the three ways below
+// to read them (4, 8 or 16 bytes a lane) meet no bank twice.
+__device__ __forceinline__ int swizzle(int row) {
+  return ((row & 1) << 2) | (row & 2) | ((row >> 2) & 1);
+}
 
 // The stages of a chunk that fall to a warp.
 __device__ __forceinline__ void part_of(const MmaPlan& p, int chunk, int part, int* first, int* end) {
@@ -406,34 +407,31 @@ __device__ __forceinline__ void part_of(const MmaPlan& p, int chunk, int part, i
 // The scales and zero points of a stage's groups in one row, as they are held.
 template <int kGroups>
 struct HeldScales {
-  uint32_t s[(kGroups + 1) / 2];
-  uint32_t z;
+  uint32_t s[kGroups];            // two scales each
+  uint32_t z[(kGroups + 1) / 2];  // four zero points each (kGroups = 1: two)
 };
 
 // kCols: columns of the matrix instruction in tiles of 8 (kTiles of them);
 // kParts: fp16 parts of a vector.  With kTiles = 1 and two parts, columns 0-3
 // hold the high parts of 4 vectors and 4-7 the low ones; otherwise the tiles'
-// first half holds the high parts.  kGroups: groups in a stage (128 / group).
+// first half holds the high parts.  kGroups: groups in half a stage (128 / group).
 template <class T, int kTiles, int kParts, int kGroups, bool kZeros>
 __global__ void __launch_bounds__(kMmaThreads, 1)
     products_kernel(Q4View v, Q4Range r, const T* x, int batch, int64_t ldx, Q4Out o, MmaPlan p) {
   constexpr bool kPacked = kTiles == 1 && kParts == 2;
   constexpr int kOutTiles = kPacked ? 1 : kTiles / kParts;
-  constexpr int kOutCols = 8 * kOutTiles;
   constexpr int kPerGroup = 4 / kGroups;  // words of 8 codes a lane has in a group
   extern __shared__ __align__(16) uint8_t raw[];
   __shared__ MmaShared sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
   uint8_t* ring = raw + warp * (kRing * kStageBytes4);
-  constexpr int kScales = kGroups * kTileRows4;  // words of a stage's scales
+  constexpr int kScales = 2 * kGroups * kTileRows4;  // words of a stage's scales
   uint32_t* scales = reinterpret_cast<uint32_t*>(raw + kMmaWarps * kRing * kStageBytes4) +
-                     warp * (2 * kScales * (kZeros ? 2 : 1));
-  float* sums = reinterpret_cast<float*>(raw + kMmaWarps * kRing * kStageBytes4 +
-                                         kMmaWarps * 2 * kScales * (kZeros ? 2 : 1) * 4);
-  uint4* vectors = reinterpret_cast<uint4*>(
-      reinterpret_cast<uint8_t*>(sums) +
-      (p.split > 1 ? kMmaWarps * kOutCols * kSumStride * sizeof(float) : 0));
+                     warp * (2 * kScales);
+  float* sums = reinterpret_cast<float*>(raw + kMmaWarps * (kRing * kStageBytes4 + 2 * kScales * 4));
+  const int sum_words = batch * kSumStride;  // of a warp
+  uint4* vectors = reinterpret_cast<uint4*>(sums + (p.split > 1 ? kMmaWarps * sum_words : 0));
   const int slots = kMmaWarps / p.split, slot = warp / p.split, part = warp % p.split;
 
   if (threadIdx.x < kQ4SearchBatch) sh.largest[threadIdx.x] = 0;
@@ -444,6 +442,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   auto tile_of = [&](int iteration) {
     return (static_cast<int64_t>(iteration) * slots + slot) * gridDim.x + blockIdx.x;
   };
+  const int64_t stride = static_cast<int64_t>(slots) * gridDim.x;
+  const int mine = static_cast<int>((p.tiles - tile_of(0) + stride - 1) / stride);  // this slot's tiles
   // this lane's row of a tile, as a row number in the pools; -1: none
   auto row_of = [&](int iteration) -> int32_t {
     const int64_t i = tile_of(iteration) * kTileRows4 + lane;
@@ -462,9 +462,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   const uint8_t* from[4];
   int64_t scales_at = 0;
   bool some = false;  // the tile has rows
-  const bool together = v.groups % kGroups == 0 &&
-                        reinterpret_cast<uintptr_t>(v.scales) % (2 * kGroups) == 0 &&
-                        (!kZeros || reinterpret_cast<uintptr_t>(v.zeros) % kGroups == 0);
+  const bool together = v.groups % (2 * kGroups) == 0 &&
+                        reinterpret_cast<uintptr_t>(v.scales) % (4 * kGroups) == 0 &&
+                        (!kZeros || reinterpret_cast<uintptr_t>(v.zeros) % (2 * kGroups) == 0);
   auto enter_tile = [&]() {
     const int32_t row = row_after;
     sh.rows[warp][next_iteration & 3][lane] = row;
@@ -475,45 +475,54 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     const int32_t read = row >= 0 ? row : some ? first : 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      from[i] = v.codes + static_cast<int64_t>(__shfl_sync(0xffffffffu, read, g + 8 * i)) * v.width + 16 * t;
+      from[i] = v.codes + static_cast<int64_t>(__shfl_sync(0xffffffffu, read, g + 8 * i)) * v.width;
     scales_at = static_cast<int64_t>(__shfl_sync(0xffffffffu, read, g + 8 * t)) * v.groups;
   };
   enter_tile();
   const int quarters = v.width >> 4;  // 16-byte pieces of a row
-  const int to_lane = g * 64 + ((t ^ swizzle(g)) << 4);
+  const int to_lane = g * 128 + ((t ^ swizzle(g)) << 4);
   HeldScales<kGroups> held;
   auto send = [&](uint8_t* to) {
-    if (next_iteration < p.iterations) {
-      const bool valid = some && 4 * next_stage + t < quarters;
-      const uint32_t ahead = valid ? 64u * next_stage : 0u;
+    if (next_iteration < mine) {
+      const uint32_t ahead = 128u * next_stage + 16u * t;
+      const bool near = some && 8 * next_stage + t < quarters;
+      const bool far = some && 8 * next_stage + 4 + t < quarters;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) copy_ahead(to + to_lane + i * 512, from[i] + ahead, valid);
-      const int64_t j = scales_at + kGroups * next_stage;
+      for (int i = 0; i < 4; ++i) {
+        // of what lies behind the row nothing is read, and zeros are written
+        copy_ahead(to + to_lane + i * 1024, from[i] + (near ? ahead : 0u), near);
+        copy_ahead(to + (to_lane ^ 64) + i * 1024, from[i] + (far ? ahead + 64u : 0u), far);
+      }
+      const int64_t j = scales_at + 2 * kGroups * next_stage;
       held = {};
       if (!some) {
-      } else if (kGroups == 1 || together) {
-        if constexpr (kGroups == 1) held.s[0] = v.scales[j];
-        if constexpr (kGroups == 2) held.s[0] = *reinterpret_cast<const uint32_t*>(v.scales + j);
+      } else if (together) {
+        if constexpr (kGroups == 1) held.s[0] = *reinterpret_cast<const uint32_t*>(v.scales + j);
+        if constexpr (kGroups == 2)
+          *reinterpret_cast<uint2*>(held.s) = *reinterpret_cast<const uint2*>(v.scales + j);
         if constexpr (kGroups == 4) {
-          const uint2 u = *reinterpret_cast<const uint2*>(v.scales + j);
-          held.s[0] = u.x, held.s[kGroups / 4] = u.y;
+          const uint4 u = *reinterpret_cast<const uint4*>(v.scales + j);
+          held.s[0] = u.x, held.s[1] = u.y, held.s[2] = u.z, held.s[3] = u.w;
         }
-        if constexpr (kZeros && kGroups == 1) held.z = v.zeros[j];
-        if constexpr (kZeros && kGroups == 2) held.z = *reinterpret_cast<const uint16_t*>(v.zeros + j);
-        if constexpr (kZeros && kGroups == 4) held.z = *reinterpret_cast<const uint32_t*>(v.zeros + j);
+        if constexpr (kZeros && kGroups == 1) held.z[0] = *reinterpret_cast<const uint16_t*>(v.zeros + j);
+        if constexpr (kZeros && kGroups == 2) held.z[0] = *reinterpret_cast<const uint32_t*>(v.zeros + j);
+        if constexpr (kZeros && kGroups == 4) {
+          const uint2 u = *reinterpret_cast<const uint2*>(v.zeros + j);
+          held.z[0] = u.x, held.z[1] = u.y;
+        }
       } else {
 #pragma unroll
-        for (int e = 0; e < kGroups; ++e)
-          if (kGroups * next_stage + e < v.groups) {
+        for (int e = 0; e < 2 * kGroups; ++e)
+          if (2 * kGroups * next_stage + e < v.groups) {
             held.s[e >> 1] |= static_cast<uint32_t>(v.scales[j + e]) << (16 * (e & 1));
-            if (kZeros) held.z |= static_cast<uint32_t>(v.zeros[j + e]) << (8 * e);
+            if (kZeros) held.z[e >> 2] |= static_cast<uint32_t>(v.zeros[j + e]) << (8 * (e & 3));
           }
       }
       if (++next_stage == next_end) {
         do {
           if (++next_chunk == p.chunks) {
             next_chunk = 0;
-            if (++next_iteration < p.iterations) enter_tile();
+            if (++next_iteration < mine) enter_tile();
           }
           part_of(p, next_chunk, part, &next_stage, &next_end);
         } while (next_stage == next_end);
@@ -522,17 +531,20 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     copy_close();
   };
   // Puts the scales that came with the last stage sent where every lane of the
-  // warp finds those of its four rows side by side, as fp32, and 1024 + zero
-  // point, twice, in fp16.
+  // warp finds those of its four rows side by side: as fp32, or with zero
+  // points as they are held, below 1024 + zero in fp16.
   auto put_scales = [&](uint32_t* to) {
 #pragma unroll
-    for (int j = 0; j < kGroups; ++j) {
+    for (int j = 0; j < 2 * kGroups; ++j) {
       const uint32_t bits = (held.s[j >> 1] >> (16 * (j & 1))) & 0xffffu;
-      const float as_half = __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
-      to[j * kTileRows4 + lane] = v.scale_bf16 ? bits << 16 : __float_as_uint(as_half);
-      if (kZeros)
-        to[2 * kScales + j * kTileRows4 + lane] =
-            0x64006400u + ((held.z >> (8 * j)) & 15u) * 0x00010001u;
+      uint32_t word;
+      if (kZeros) {
+        word = bits | ((held.z[j >> 2] >> (8 * (j & 3))) & 15u) << 16 | 0x64000000u;
+      } else {
+        word = __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(bits))));
+        if (v.scale_bf16) word = bits << 16;
+      }
+      to[j * kTileRows4 + lane] = word;
     }
   };
   // ---- the vectors' scales
@@ -567,7 +579,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     const int first = chunk * p.chunk_stages;
     int len = p.stages - first;
     if (len > p.chunk_stages) len = p.chunk_stages;
-    for (int item = threadIdx.x; item < len * 4 * kTiles * 32; item += kMmaThreads) {
+    for (int item = threadIdx.x; item < len * 8 * kTiles * 32; item += kMmaThreads) {
       const int l = item & 31, tile = (item >> 5) % kTiles, word = (item >> 5) / kTiles;
       const int w = word & 3, column = l >> 2, q = l & 3;
       int b, low;
@@ -576,7 +588,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       } else {
         b = (tile % kOutTiles) * 8 + column, low = tile / kOutTiles;
       }
-      int k = kStageCodes * (first + (word >> 2));
+      int k = kStageCodes * first + 128 * (word >> 2);
       if constexpr (kGroups == 4) k += 32 * w + 8 * q;
       else if constexpr (kGroups == 2) k += 64 * (w >> 1) + 16 * q + 8 * (w & 1);
       else k += 32 * q + 8 * w;
@@ -621,12 +633,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   send(ring);
   put_scales(scales);
   send(ring + kStageBytes4);
-  static_assert(kRing == 3, "the stage at hand, the next, and the one being sent");
 
   __syncthreads();
 
-  uint32_t ring_at = 0, ring_free = (kRing - 1) * kStageBytes4;  // bytes into the ring
-  uint32_t scales_now = 0;                                       // words into the scales
+  uint32_t ring_at = 0;     // bytes into the ring
+  uint32_t scales_now = 0;  // words into the scales
   for (int iteration = 0; iteration < p.iterations; ++iteration) {
     float total[2][kOutTiles][4] = {};
     for (int chunk = 0; chunk < p.chunks; ++chunk) {
@@ -637,97 +648,111 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       }
       int stage, end;
       part_of(p, chunk, part, &stage, &end);
-      const uint4* vec = vectors + (stage - chunk * p.chunk_stages) * (4 * kTiles * 32) + lane;
+      if (iteration >= mine) end = stage;
+      const uint4* vec = vectors + (stage - chunk * p.chunk_stages) * (8 * kTiles * 32) + lane;
 #pragma unroll 1
-      for (; stage < end; ++stage, vec += 4 * kTiles * 32) {
-        copy_wait<kRing - 2>();
+      for (; stage < end; ++stage, vec += 8 * kTiles * 32) {
+        copy_wait<1>();
         __syncwarp();
-        const uint32_t* scale_row = scales + scales_now + 4 * g;
-        scales_now ^= kScales;
-        put_scales(scales + scales_now);  // of the next stage
-        send(ring + ring_free);
-        const uint8_t* codes = ring + ring_at + g * 64;
-        ring_free = ring_at;
-        ring_at = ring_at == (kRing - 1) * kStageBytes4 ? 0 : ring_at + kStageBytes4;
-
-        uint32_t words[4][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint8_t* c = codes + i * 512;
-          if constexpr (kGroups == 4) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              words[i][j] = *reinterpret_cast<const uint32_t*>(c + ((j ^ swizzle(g)) << 4) + 4 * t);
-          } else if constexpr (kGroups == 2) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const uint2 u = *reinterpret_cast<const uint2*>(
-                  c + (((2 * j + (t >> 1)) ^ swizzle(g)) << 4) + 8 * (t & 1));
-              words[i][2 * j] = u.x;
-              words[i][2 * j + 1] = u.y;
-            }
-          } else {
-            const uint4 u = *reinterpret_cast<const uint4*>(c + ((t ^ swizzle(g)) << 4));
-            words[i][0] = u.x, words[i][1] = u.y, words[i][2] = u.z, words[i][3] = u.w;
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < kGroups; ++j) {
-          float acc[2][kTiles][4];
-          uint32_t one[4], sixteen[4];
-          const float4 s4 = *reinterpret_cast<const float4*>(scale_row + j * kTileRows4);
-          const float scale[4] = {s4.x, s4.y, s4.z, s4.w};
-          uint4 z4 = make_uint4(0x64086408u, 0x64086408u, 0x64086408u, 0x64086408u);
-          if (kZeros) z4 = *reinterpret_cast<const uint4*>(scale_row + 2 * kScales + j * kTileRows4);
-          one[0] = z4.x, one[1] = z4.y, one[2] = z4.z, one[3] = z4.w;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sixteen[i] = ((one[i] & 0x000f000fu) << 4) | 0xd400d400u;  // -(64 + zero)
-#pragma unroll
-          for (int w = j * kPerGroup; w < (j + 1) * kPerGroup; ++w) {
-            uint32_t a[4][4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t u = words[i][w], far = u >> 8;
-              a[i][0] = sub2(and_or(u, 0x000f000fu, 0x64006400u), one[i]);
-              a[i][1] = sixteenth2(and_or(u, 0x00f000f0u, 0x64006400u), sixteen[i]);
-              a[i][2] = sub2(and_or(far, 0x000f000fu, 0x64006400u), one[i]);
-              a[i][3] = sixteenth2(and_or(far, 0x00f000f0u, 0x64006400u), sixteen[i]);
-            }
-#pragma unroll
-            for (int c = 0; c < kTiles; ++c) {
-              const uint4 b = vec[(w * kTiles + c) * 32];
-#pragma unroll
-              for (int m = 0; m < 2; ++m) {
-                float(&d)[4] = acc[m][c];
-                if (w == j * kPerGroup)
-                  mma_16816(d, a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], b.x, b.y,
-                            0.0f, 0.0f, 0.0f, 0.0f);
-                else
-                  mma_16816(d, a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], b.x, b.y,
-                            d[0], d[1], d[2], d[3]);
-                mma_16816(d, a[2 * m][2], a[2 * m + 1][2], a[2 * m][3], a[2 * m + 1][3], b.z, b.w,
-                          d[0], d[1], d[2], d[3]);
-              }
-            }
-          }
+        for (int half = 0; half < 2; ++half) {
+          const uint8_t* codes = ring + ring_at + g * 128;
+          uint32_t words[4][4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int m = i >> 1, h = 2 * (i & 1);
+            const uint8_t* c = codes + i * 1024;
+            if constexpr (kGroups == 4) {
 #pragma unroll
-            for (int c = 0; c < kOutTiles; ++c)
+              for (int j = 0; j < 4; ++j)
+                words[i][j] = *reinterpret_cast<const uint32_t*>(
+                    c + (((4 * half + j) ^ swizzle(g)) << 4) + 4 * t);
+            } else if constexpr (kGroups == 2) {
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                float sum = acc[m][c][h + e];
-                if constexpr (!kPacked && kParts == 2) sum += acc[m][c + kOutTiles][h + e];
-                total[m][c][h + e] = fmaf(scale[i], sum, total[m][c][h + e]);
+              for (int j = 0; j < 2; ++j) {
+                const uint2 u = *reinterpret_cast<const uint2*>(
+                    c + (((4 * half + 2 * j + (t >> 1)) ^ swizzle(g)) << 4) + 8 * (t & 1));
+                words[i][2 * j] = u.x;
+                words[i][2 * j + 1] = u.y;
               }
+            } else {
+              const uint4 u = *reinterpret_cast<const uint4*>(c + (((4 * half + t) ^ swizzle(g)) << 4));
+              words[i][0] = u.x, words[i][1] = u.y, words[i][2] = u.z, words[i][3] = u.w;
+            }
+          }
+          const uint32_t* scale_row = scales + scales_now + half * (kGroups * kTileRows4) + 4 * g;
+          if (half == 1) {
+            // the codes of this stage are in registers: the one after the next
+            // takes their place
+            __syncwarp();
+            scales_now ^= kScales;
+            put_scales(scales + scales_now);
+            send(ring + ring_at);
+            ring_at ^= kStageBytes4;
+            if (kStageCodes * stage + 128 >= v.dim) continue;
+          }
+#pragma unroll
+          for (int j = 0; j < kGroups; ++j) {
+            float acc[2][kTiles][4], scale[4];
+            uint32_t one[4], sixteen[4];
+            const uint4 s4 = *reinterpret_cast<const uint4*>(scale_row + j * kTileRows4);
+            const uint32_t held4[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if constexpr (kZeros) {
+                scale[i] = __half2float(__ushort_as_half(static_cast<unsigned short>(held4[i])));
+                if (v.scale_bf16) scale[i] = __uint_as_float(held4[i] << 16);
+                one[i] = __byte_perm(held4[i], 0, 0x3232);                     // 1024 + zero
+                sixteen[i] = ((one[i] & 0x000f000fu) << 4) | 0xd400d400u;      // -(64 + zero)
+              } else {
+                scale[i] = __uint_as_float(held4[i]);
+                one[i] = 0x64086408u;
+                sixteen[i] = 0xd480d480u;
+              }
+            }
+#pragma unroll
+            for (int w = j * kPerGroup; w < (j + 1) * kPerGroup; ++w) {
+              uint32_t a[4][4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t u = words[i][w], far = u >> 8;
+                a[i][0] = sub2(and_or(u, 0x000f000fu, 0x64006400u), one[i]);
+                a[i][1] = sixteenth2(and_or(u, 0x00f000f0u, 0x64006400u), sixteen[i]);
+                a[i][2] = sub2(and_or(far, 0x000f000fu, 0x64006400u), one[i]);
+                a[i][3] = sixteenth2(and_or(far, 0x00f000f0u, 0x64006400u), sixteen[i]);
+              }
+#pragma unroll
+              for (int c = 0; c < kTiles; ++c) {
+                const uint4 b = vec[((4 * half + w) * kTiles + c) * 32];
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                  float(&d)[4] = acc[m][c];
+                  if (w == j * kPerGroup)
+                    mma_16816(d, a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], b.x,
+                              b.y, 0.0f, 0.0f, 0.0f, 0.0f);
+                  else
+                    mma_16816(d, a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], b.x,
+                              b.y, d[0], d[1], d[2], d[3]);
+                  mma_16816(d, a[2 * m][2], a[2 * m + 1][2], a[2 * m][3], a[2 * m + 1][3], b.z, b.w,
+                            d[0], d[1], d[2], d[3]);
+                }
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int m = i >> 1, h = 2 * (i & 1);
+#pragma unroll
+              for (int c = 0; c < kOutTiles; ++c)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  float sum = acc[m][c][h + e];
+                  if constexpr (!kPacked && kParts == 2) sum += acc[m][c + kOutTiles][h + e];
+                  total[m][c][h + e] = fmaf(scale[i], sum, total[m][c][h + e]);
+                }
+            }
           }
         }
       }
     }
-    int32_t rows[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) rows[i] = sh.rows[warp][iteration & 3][g + 8 * i];
     if constexpr (kPacked) {  // the low parts' columns are two lanes on
 #pragma unroll
       for (int m = 0; m < 2; ++m)
@@ -737,17 +762,36 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     }
     const int64_t first = tile_of(iteration) * kTileRows4;
     if (p.split == 1) {
+      if (iteration >= mine) continue;
+      int32_t rows[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rows[i] = sh.rows[warp][iteration & 3][g + 8 * i];
+      const bool whole = __all_sync(0xffffffffu, (rows[0] | rows[1] | rows[2] | rows[3]) >= 0);
+      if (whole && o.mode == kStore && o.dtype == KNN_DTYPE_F32) {
+#pragma unroll
+        for (int c = 0; c < kOutTiles; ++c)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int b = 8 * c + 2 * t + e;
+            if (b >= batch || (kPacked && t >= 2)) continue;
+            float* y = static_cast<float*>(o.y) + b * o.ld + first + g;
+            const float f = sh.inverse[b];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[8 * i] = total[i >> 1][c][2 * (i & 1) + e] * f;
+          }
+        continue;
+      }
 #pragma unroll
       for (int c = 0; c < kOutTiles; ++c)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int b = 8 * c + 2 * t + e;
-          const bool mine = b < batch && (!kPacked || t < 2);
+          const bool mine_too = b < batch && (!kPacked || t < 2);
           uint32_t least = kNoKey;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int64_t at = first + g + 8 * i;
-            if (!mine || at >= r.count) continue;
+            if (!mine_too || at >= r.count) continue;
             float y = total[i >> 1][c][2 * (i & 1) + e] * sh.inverse[b];
             if (rows[i] < 0) y = at < n ? __int_as_float(0x7fc00000) : 0.0f;
             const float key = put(o, b, at, y, o.mode == kKeyL2 && rows[i] >= 0 ? v.norms[rows[i]] : 0.0f);
@@ -757,28 +801,31 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1)
               least = min(least, __shfl_xor_sync(0xffffffffu, least, d));
-            if (g == 0 && mine && first < r.count) o.minima[b * p.tiles + first / kTileRows4] = least;
+            if (g == 0 && mine_too) o.minima[b * p.tiles + first / kTileRows4] = least;
           }
         }
     } else {
-      float* mine = sums + warp * (kOutCols * kSumStride);
+      float* own = sums + warp * sum_words;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int c = 0; c < kOutTiles; ++c)
 #pragma unroll
-        for (int c = 0; c < kOutTiles; ++c)
+        for (int e = 0; e < 2; ++e) {
+          const int b = 8 * c + 2 * t + e;
+          if (b >= batch || (kPacked && t >= 2)) continue;
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            mine[(8 * c + 2 * t + e) * kSumStride + g + 8 * i] = total[i >> 1][c][2 * (i & 1) + e];
-      }
+          for (int i = 0; i < 4; ++i)
+            own[b * kSumStride + g + 8 * i] = total[i >> 1][c][2 * (i & 1) + e];
+        }
       __syncthreads();
       // a warp to a tile and vector, a lane to a row
       for (int item = warp; item < slots * batch; item += kMmaWarps) {
         const int s = item / batch, b = item - s * batch;
         const int64_t tile = (static_cast<int64_t>(iteration) * slots + s) * gridDim.x + blockIdx.x;
+        if (tile >= p.tiles) continue;
         const int64_t at = tile * kTileRows4 + lane;
         float y = 0.0f;
         for (int q = 0; q < p.split; ++q)
-          y += sums[((s * p.split + q) * kOutCols + b) * kSumStride + lane];
+          y += sums[(s * p.split + q) * sum_words + b * kSumStride + lane];
         y *= sh.inverse[b];
         const int32_t at_row = sh.rows[s * p.split][iteration & 3][lane];
         if (at_row < 0) y = at < n ? __int_as_float(0x7fc00000) : 0.0f;
@@ -789,7 +836,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         }
         if (o.minima) {
           least = __reduce_min_sync(0xffffffffu, least);
-          if (lane == 0 && tile < p.tiles) o.minima[b * p.tiles + tile] = least;
+          if (lane == 0) o.minima[b * p.tiles + tile] = least;
         }
       }
       __syncthreads();
@@ -1008,10 +1055,9 @@ unsigned row_grid(int64_t rows) {
 }
 
 // Shared memory of a block beside the vectors.
-int64_t mma_fixed_bytes(int split, int out_cols, int groups, bool zeros) {
-  return kMmaWarps * kRing * kStageBytes4 +
-         kMmaWarps * 2 * groups * kTileRows4 * 4 * (zeros ? 2 : 1) +
-         (split > 1 ? kMmaWarps * out_cols * kSumStride * 4 : 0);
+int64_t mma_fixed_bytes(int split, int batch, int groups) {
+  return kMmaWarps * (kRing * kStageBytes4 + 2 * 2 * groups * kTileRows4 * 4) +
+         (split > 1 ? kMmaWarps * batch * kSumStride * 4 : 0);
 }
 
 // Warps that share a tile: the number with the least time of a block, in
@@ -1031,7 +1077,6 @@ int mma_split(int64_t tiles, int stages, int sms) {
 template <class T, int kTiles, int kParts, int kGroups, bool kZeros>
 cudaError_t products(const Q4View& v, const Q4Range& r, const T* x, int batch, int64_t ldx,
                      const Q4Out& o, cudaStream_t stream) {
-  constexpr int kOutCols = kTiles == 1 ? 8 : 8 * kTiles / kParts;
   constexpr int64_t kMost = 232448 - sizeof(MmaShared) - 64;
   auto kernel = products_kernel<T, kTiles, kParts, kGroups, kZeros>;
   const int sms = store_sm_count();
@@ -1039,14 +1084,14 @@ cudaError_t products(const Q4View& v, const Q4Range& r, const T* x, int batch, i
   p.tiles = (r.count + kTileRows4 - 1) / kTileRows4;
   p.stages = static_cast<int32_t>((v.dim + kStageCodes - 1) / kStageCodes);
   p.split = mma_split(p.tiles, p.stages, sms);
-  const int64_t room = (kMost - mma_fixed_bytes(2, kOutCols, kGroups, kZeros)) / (4 * kTiles * 512);
+  const int64_t room = (kMost - mma_fixed_bytes(p.split, batch, kGroups)) / (8 * kTiles * 512);
   p.chunk_stages = static_cast<int32_t>(std::min<int64_t>(p.stages, room));
   while (p.split > p.chunk_stages) p.split /= 2;  // every warp has a stage of every full chunk
   p.chunks = (p.stages + p.chunk_stages - 1) / p.chunk_stages;
   const int64_t grid = std::min<int64_t>(p.tiles, sms);
   const int64_t slots = kMmaWarps / p.split;
   p.iterations = static_cast<int32_t>((p.tiles + grid * slots - 1) / (grid * slots));
-  const size_t smem = mma_fixed_bytes(p.split, kOutCols, kGroups, kZeros) + p.chunk_stages * (4 * kTiles * 512);
+  const size_t smem = mma_fixed_bytes(p.split, batch, kGroups) + p.chunk_stages * (8 * kTiles * 512);
   static std::atomic<uint64_t> allowed{0};
   if (cudaError_t e = allow_smem(kernel, static_cast<int>(kMost), &allowed)) return e;
   store_count_launches(1);
