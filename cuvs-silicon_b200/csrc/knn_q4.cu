@@ -114,22 +114,24 @@ __device__ __forceinline__ int64_t list_row(const Q4View& v, const Q4List& l, co
 }
 
 // ------------------------------------------------------------------- pack
-// q / t to the nearest whole number, ties to even, exactly: the quotient in
-// fp32 can fall on a tie that the true one only comes near to, so the
-// remainder (exact in one fma: q and t have at most 24 and 11 bits and the
-// quotient 5) decides.
-__device__ __forceinline__ float nearest(float q, float t) {
-  float n = rintf(q / t);
-  if (fabsf(n) > 64.0f) return n;  // clamped by the caller
-  const float left = fmaf(-n, t, q), half = 0.5f * t;
-  const bool odd = (static_cast<int>(n) & 1) != 0;
-  if (left > half || (left == half && odd)) n += 1.0f;
-  else if (left < -half || (left == -half && odd)) n -= 1.0f;
+// v / s to the nearest whole number, ties to even, exactly, for s > 0 and
+// quotients below 2^20.  over is 1 / s in fp32, so the product can be one off
+// near a tie; the remainder, exact in one fma (24 + 11 bits and a quotient of
+// 5), tells.
+__device__ __forceinline__ float nearest(float v, float s, float over) {
+  constexpr float kWhole = 12582912.0f;  // 1.5 * 2^23: adding it rounds to whole numbers
+  float n = __fadd_rn(__fmaf_rn(v, over, kWhole), -kWhole);
+  const float left = fmaf(-n, s, v), half = 0.5f * s;
+  if (fabsf(left) >= half) {  // rare
+    const bool odd = (static_cast<int>(n) & 1) != 0;
+    if (fabsf(left) > half || odd) n += copysignf(1.0f, left);
+  }
   return n;
 }
 
-// One warp a row; a lane holds 4 neighbouring values of each 128.  HBM bound:
-// the values are read once, codes and scales written once.
+// One warp a row; a lane holds 8 neighbouring values of each 256, so that its
+// codes are one word.  HBM bound: values are read once, codes and scales
+// written once.
 template <class T>
 __global__ void __launch_bounds__(kThreads) pack_kernel(Q4View v, Q4List l, const T* x, int64_t ld,
                                                         bool vec) {
@@ -138,43 +140,39 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(Q4View v, Q4List l, cons
   if (l.seqs && !l.status[kStatusApplied]) return;
   if (!open_list(l, sm)) return;  // as the call that made room found it
   const int lane = threadIdx.x & 31;
-  const int span = v.group / 4;  // lanes of a group
+  const int span = v.group / 8;  // lanes of a group
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); t < l.total;
        t += static_cast<int64_t>(gridDim.x) * kWarps) {
     const int64_t row = list_row(v, l, sm, t);
     if (row < 0) continue;
     const T* in = x + t * ld;
     float norm = 0.0f;
-    for (int64_t base = 0; base < 2 * v.width; base += 128) {
-      const int64_t j = base + 4 * lane;
-      float a[4];
-      if (vec && j + 4 <= v.dim) {
-        if constexpr (sizeof(T) == 4) {
-          const float4 f = *reinterpret_cast<const float4*>(in + j);
-          a[0] = f.x, a[1] = f.y, a[2] = f.z, a[3] = f.w;
-        } else {
-          T h[4];
-          *reinterpret_cast<uint2*>(h) = *reinterpret_cast<const uint2*>(in + j);
+#pragma unroll 2
+    for (int base = 0; base < 2 * v.width; base += 256) {
+      const int j = base + 8 * lane;
+      float a[8];
+      if (vec && j + 8 <= v.dim) {
+        __align__(16) T h[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) a[e] = load_value(h + e);
-        }
+        for (int e = 0; e < static_cast<int>(sizeof(T)) / 2; ++e)
+          reinterpret_cast<uint4*>(h)[e] = __ldcs(reinterpret_cast<const uint4*>(in + j) + e);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] = load_value(h + e);
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = j + e < v.dim ? load_value(in + j + e) : 0.0f;
+        for (int e = 0; e < 8; ++e) a[e] = j + e < v.dim ? load_value(in + j + e) : 0.0f;
       }
-      float low, high;
-      if (v.zeros) {
-        high = max_nan(max_nan(max_nan(a[0], a[1]), max_nan(a[2], a[3])), 0.0f);
-        low = -max_nan(max_nan(max_nan(-a[0], -a[1]), max_nan(-a[2], -a[3])), 0.0f);
-      } else {
-        high = max_nan(max_nan(fabsf(a[0]), fabsf(a[1])), max_nan(fabsf(a[2]), fabsf(a[3])));
-        low = 0.0f;
+      float low = 0.0f, high = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        high = max_nan(high, v.zeros ? a[e] : fabsf(a[e]));
+        if (v.zeros) low = max_nan(low, -a[e]);
       }
       for (int d = 1; d < span; d <<= 1) {
         high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, d));
-        if (v.zeros) low = -max_nan(-low, -__shfl_xor_sync(0xffffffffu, low, d));
+        if (v.zeros) low = max_nan(low, __shfl_xor_sync(0xffffffffu, low, d));
       }
-      const float wide = v.zeros ? __fdiv_rn(high - low, 15.0f) : __fdiv_rn(high, 7.0f);
+      const float wide = v.zeros ? __fdiv_rn(high + low, 15.0f) : __fdiv_rn(high, 7.0f);
       uint16_t bits;
       float s;
       if (v.scale_bf16) {
@@ -186,24 +184,28 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(Q4View v, Q4List l, cons
         bits = __half_as_ushort(h);
         s = __half2float(h);
       }
+      // a scale of 0, or one that is no finite number: all values at the zero point
       const bool usable = s > 0.0f && s < __int_as_float(0x7f800000);
+      // bf16 scales can be so small that 1 / s overflows: then all of it times 2^100
+      const float up = v.scale_bf16 && s < 0x1p-100f ? 0x1p100f : 1.0f;
+      const float big = s * up, over = __fdiv_rn(1.0f, big);
       float zero = 8.0f;
-      if (v.zeros) zero = usable ? fminf(fmaxf(nearest(-low, s), 0.0f), 15.0f) : 0.0f;
+      if (v.zeros) zero = usable ? fminf(fmaxf(nearest(low * up, big, over), 0.0f), 15.0f) : 0.0f;
       uint32_t packed = 0;
-      int square = 0;
+      float square = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < 8; ++e) {
         float c = zero;
-        if (usable) c = fminf(fmaxf(nearest(a[e], s) + zero, 0.0f), 15.0f);
-        const int code = j + e < v.dim ? static_cast<int>(c) : 0;
-        const int d = j + e < v.dim ? code - static_cast<int>(zero) : 0;
-        square += d * d;
-        packed |= static_cast<uint32_t>(code) << (4 * e);
+        if (usable) c = fminf(fmaxf(nearest(a[e] * up, big, over) + zero, 0.0f), 15.0f);
+        if (j + e >= v.dim) c = 0.0f;
+        const float d = j + e < v.dim ? c - zero : 0.0f;
+        square = fmaf(d, d, square);
+        // 2^23 + c holds c in its lowest bits
+        packed |= (__float_as_uint(c + 8388608.0f) & 15u) << (4 * e);
       }
-      norm += (s * s) * static_cast<float>(square);
+      norm = fmaf(s * s, square, norm);
       if (j < 2 * v.width)
-        *reinterpret_cast<uint16_t*>(const_cast<uint8_t*>(v.codes) + row * v.width + j / 2) =
-            static_cast<uint16_t>(packed);
+        *reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(v.codes) + row * v.width + j / 2) = packed;
       if (lane % span == 0 && j < v.dim) {
         const int64_t g = row * v.groups + j / v.group;
         const_cast<uint16_t*>(v.scales)[g] = bits;
@@ -232,23 +234,24 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Q4View v, Q4List l, floa
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); t < l.total;
        t += static_cast<int64_t>(gridDim.x) * kWarps) {
     const int64_t row = list_row(v, l, sm, t);
-    for (int64_t j = 4 * lane; j < v.dim; j += 128) {
-      float a[4];
-      if (row < 0) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = __int_as_float(0x7fc00000);
-      } else {
-        const uint32_t packed = *reinterpret_cast<const uint16_t*>(v.codes + row * v.width + j / 2);
-        const int g = static_cast<int>(j / v.group);
-        const float s = scale_of(v, row, g);
-        const int z = zero_of(v, row, g);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          a[e] = static_cast<float>(static_cast<int>((packed >> (4 * e)) & 15) - z) * s;
+    const uint8_t* codes = v.codes + (row < 0 ? 0 : row) * v.width;
+#pragma unroll 4
+    for (int j = 4 * lane; j < v.dim; j += 128) {
+      const uint32_t packed = *reinterpret_cast<const uint16_t*>(codes + j / 2);
+      const int g = j / v.group;
+      float s = __int_as_float(0x7fc00000);  // no page: NaN
+      int z = 8;
+      if (row >= 0) {
+        s = scale_of(v, row, g);
+        z = zero_of(v, row, g);
       }
+      float a[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        a[e] = static_cast<float>(static_cast<int>((packed >> (4 * e)) & 15) - z) * s;
       float* o = out + t * ld + j;
       if (vec && j + 4 <= v.dim) {
-        *reinterpret_cast<float4*>(o) = make_float4(a[0], a[1], a[2], a[3]);
+        __stcs(reinterpret_cast<float4*>(o), make_float4(a[0], a[1], a[2], a[3]));
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -853,62 +856,127 @@ constexpr int kMaxCandidates = KNN_MAX_K + kMoreCandidates;
 constexpr int kGroupCap = 1024;
 constexpr int kCandCap = 4096;
 
+constexpr int kBins = 2048;
+constexpr int kMinimaHeld = 32;  // minima that a thread keeps in registers
+
 struct SelectSmem {
   uint64_t cand[kCandCap];
   uint64_t final_key[kMaxCandidates];
   uint32_t final_row[kMaxCandidates];
-  uint32_t hist[256];
+  uint32_t hist[kBins];
+  uint32_t part[32];
   int32_t group[kGroupCap];
   uint32_t count, groups;
   uint64_t prefix;
   int64_t rank;
 };
 
-// The value of rank `rank` (from 0) among load(0 .. n - 1), by 8 bits a pass
-// from the top; kBits 32 or 64.
-template <int kBits, class Load>
+// Adds one to the bin of each thread that has one (bin < kBins).  Keys share
+// their leading bits: a warp adds up equal bins first.
+__device__ __forceinline__ void count_bin(SelectSmem& sm, uint32_t bin) {
+  const uint32_t same = __match_any_sync(0xffffffffu, bin);
+  if (bin < kBins && (threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(&sm.hist[bin], __popc(same));
+}
+
+// The bin that the value of rank `rank` falls in, and (in sm.rank) its rank
+// there.  All threads; the bins are cleared for the next count.
+__device__ uint32_t find_bin(SelectSmem& sm, int64_t rank) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int kPer = kBins / kSelectThreads;
+  __syncthreads();
+  uint32_t h[kPer], sum = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    sum += h[j] = sm.hist[kPer * threadIdx.x + j];
+    sm.hist[kPer * threadIdx.x + j] = 0;
+  }
+  uint32_t inc = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const uint32_t up = __shfl_up_sync(0xffffffffu, inc, d);
+    if (lane >= d) inc += up;
+  }
+  if (lane == 31) sm.part[warp] = inc;
+  __syncthreads();
+  uint32_t before = sm.part[lane], all = before;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const uint32_t up = __shfl_up_sync(0xffffffffu, all, d);
+    if (lane >= d) all += up;
+  }
+  const uint32_t first = __shfl_sync(0xffffffffu, all - before, warp);
+  int64_t left = rank - static_cast<int64_t>(first + inc - sum);
+  if (left >= 0 && left < static_cast<int64_t>(sum)) {
+    int j = 0;
+    while (left >= static_cast<int64_t>(h[j])) left -= h[j++];
+    sm.prefix = static_cast<uint64_t>(kPer * threadIdx.x + j);
+    sm.rank = left;
+  }
+  __syncthreads();
+  return static_cast<uint32_t>(sm.prefix);
+}
+
+// The 64-bit value of rank `rank` (from 0) among load(0 .. n - 1), 11 bits a
+// pass from the top.
+template <class Load>
 __device__ uint64_t nth(int64_t n, int64_t rank, SelectSmem& sm, Load load) {
   uint64_t prefix = 0;
-  for (int shift = kBits - 8; shift >= 0; shift -= 8) {
-    __syncthreads();
-    if (threadIdx.x < 256) sm.hist[threadIdx.x] = 0;
-    __syncthreads();
-    const uint64_t above = shift == kBits - 8 ? 0 : ~0ull << (shift + 8);
+  for (int top = 64; top > 0;) {
+    const int shift = top > 11 ? top - 11 : 0;
+    const uint64_t above = top == 64 ? 0 : ~0ull << top;
+    const uint32_t mask = (1u << (top - shift)) - 1;
     for (int64_t base = 0; base < n; base += kSelectThreads) {
       const int64_t i = base + threadIdx.x;
       const uint64_t x = i < n ? load(i) : 0;
-      const bool in = i < n && (x & above) == (prefix & above);
-      const uint32_t bin = in ? static_cast<uint32_t>(x >> shift) & 255u : 256u;
-      // keys share their leading bits: add up equal bins within the warp
-      const uint32_t same = __match_any_sync(0xffffffffu, bin);
-      if (in && (threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(&sm.hist[bin], __popc(same));
+      const bool in = i < n && (x & above) == prefix;
+      count_bin(sm, in ? static_cast<uint32_t>(x >> shift) & mask : static_cast<uint32_t>(kBins));
     }
-    __syncthreads();
-    if (threadIdx.x < 32) {
-      const int lane = threadIdx.x;
-      uint32_t h[8], sum = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sum += h[j] = sm.hist[8 * lane + j];
-      uint32_t inc = sum;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const uint32_t up = __shfl_up_sync(0xffffffffu, inc, d);
-        if (lane >= d) inc += up;
-      }
-      int64_t left = rank - static_cast<int64_t>(inc - sum);
-      if (left >= 0 && left < static_cast<int64_t>(sum)) {
-        int j = 0;
-        while (left >= static_cast<int64_t>(h[j])) left -= h[j++];
-        sm.prefix = prefix | (static_cast<uint64_t>(8 * lane + j) << shift);
-        sm.rank = left;
-      }
-    }
-    __syncthreads();
-    prefix = sm.prefix;
+    prefix |= static_cast<uint64_t>(find_bin(sm, rank)) << shift;
     rank = sm.rank;
+    top = shift;
   }
   __syncthreads();
   return prefix;
+}
+
+// A bound that at least rank + 1 of the minima lie at or below, and hardly
+// more: the value of that rank with its last 10 bits set (two counts of 11
+// bits).  Up to 32 minima a thread are read once and kept.
+__device__ uint32_t minima_bound(const uint32_t* minima, int64_t groups, int64_t rank,
+                                 SelectSmem& sm) {
+  uint32_t held[kMinimaHeld];
+  const bool keep = groups <= kMinimaHeld * kSelectThreads;
+  if (keep) {
+#pragma unroll
+    for (int j = 0; j < kMinimaHeld; ++j) {
+      const int64_t i = static_cast<int64_t>(j) * kSelectThreads + threadIdx.x;
+      held[j] = i < groups ? minima[i] : kNoKey;
+    }
+  }
+  uint32_t prefix = 0;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    const int shift = pass ? 10 : 21;
+    auto count = [&](uint32_t x, bool in) {
+      in = in && (pass == 0 || (x >> 21) == (prefix >> 21));
+      count_bin(sm, in ? (x >> shift) & 2047u : static_cast<uint32_t>(kBins));
+    };
+    if (keep) {
+#pragma unroll
+      for (int j = 0; j < kMinimaHeld; ++j)
+        if (static_cast<int64_t>(j) * kSelectThreads < groups)
+          count(held[j], static_cast<int64_t>(j) * kSelectThreads + threadIdx.x < groups);
+    } else {
+#pragma unroll 4
+      for (int64_t base = 0; base < groups; base += kSelectThreads) {
+        const int64_t i = base + threadIdx.x;
+        count(i < groups ? minima[i] : kNoKey, i < groups);
+      }
+    }
+    prefix |= find_bin(sm, rank) << shift;
+    rank = sm.rank;
+  }
+  return prefix | 1023u;
 }
 
 // Sorts sm.cand[0 .. n) ascending, n a power of two.
@@ -953,10 +1021,9 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
   minima += b * groups;
   const int wanted = k + kMoreCandidates;
   uint32_t tau = kNoKey - 1;
-  if (groups > wanted) {
-    tau = static_cast<uint32_t>(nth<32>(groups, wanted - 1, sm, [&](int64_t i) { return minima[i]; }));
-    tau = min(tau, kNoKey - 1);
-  }
+  for (int i = threadIdx.x; i < kBins; i += kSelectThreads) sm.hist[i] = 0;
+  __syncthreads();
+  if (groups > wanted) tau = min(minima_bound(minima, groups, wanted - 1, sm), kNoKey - 1);
   if (threadIdx.x == 0) sm.count = sm.groups = 0;
   __syncthreads();
   for (int64_t g = threadIdx.x; g < groups; g += kSelectThreads)
@@ -982,8 +1049,10 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
     const int count = static_cast<int>(sm.count);
     int size = 2;
     while (size < count) size <<= 1;
-    for (int e = count + threadIdx.x; e < size; e += kSelectThreads) sm.cand[e] = ~0ull;
-    sort_candidates(sm, size);
+    if (count > wanted) {
+      for (int e = count + threadIdx.x; e < size; e += kSelectThreads) sm.cand[e] = ~0ull;
+      sort_candidates(sm, size);
+    }
     have = min(count, wanted);
   } else {
     // many equal keys: the row of rank wanted - 1 by (key, index), over all rows
@@ -991,7 +1060,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
       const uint32_t key = ordered(keys[i]);
       return (static_cast<uint64_t>(key) << 32) | static_cast<uint32_t>(i);
     };
-    const uint64_t last = n > wanted ? nth<64>(n, wanted - 1, sm, load) : ~0ull;
+    const uint64_t last = n > wanted ? nth(n, wanted - 1, sm, load) : ~0ull;
     __syncthreads();
     if (threadIdx.x == 0) sm.count = 0;
     __syncthreads();
@@ -1012,13 +1081,24 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
     const uint32_t i = static_cast<uint32_t>(sm.cand[e]);
     const int64_t row = v.places.at(r.seq, i);
     double sum = 0.0;
-    for (int64_t j = lane; j < v.dim; j += 32) {
-      const int g = static_cast<int>(j / v.group);
-      const int code = (v.codes[row * v.width + j / 2] >> (4 * (j & 1))) & 15;
-      const double value = static_cast<float>(code - zero_of(v, row, g)) * scale_of(v, row, g);
-      const double qv = load_value(q + j);
-      if (mode == kKeyL2) sum += (qv - value) * (qv - value);
-      else sum -= qv * value;
+#pragma unroll 4
+    for (int j = 8 * lane; j < v.dim; j += 256) {
+      const uint32_t packed = *reinterpret_cast<const uint32_t*>(v.codes + row * v.width + j / 2);
+      const int g = j / v.group;
+      const float s = scale_of(v, row, g);
+      const int z = zero_of(v, row, g);
+      float qv[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) qv[c] = j + c < v.dim ? load_value(q + j + c) : 0.0f;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const int code = static_cast<int>((packed >> (4 * c)) & 15);
+        // exact: 5 bits times 11; codes behind the last value count for nothing
+        const double value = j + c < v.dim ? static_cast<float>(code - z) * s : 0.0f;
+        const double term = static_cast<double>(qv[c]);
+        if (mode == kKeyL2) sum = fma(term - value, term - value, sum);
+        else sum = fma(-term, value, sum);
+      }
     }
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -1152,10 +1232,10 @@ cudaError_t launch_q4_pack(const Q4View& v, const Q4List& l, const void* rows, i
   store_count_launches(1);
   const unsigned grid = row_grid(l.total);
   const uintptr_t bits = reinterpret_cast<uintptr_t>(rows);
+  const bool vec = ((bits | (ld * (dtype == KNN_DTYPE_F32 ? 4 : 2))) & 15) == 0;
   if (dtype == KNN_DTYPE_F32)
     return launch_after(pack_kernel<float>, grid, kThreads, 0, stream, v, l,
-                        static_cast<const float*>(rows), ld, ((bits | (ld * 4)) & 15) == 0);
-  const bool vec = ((bits | (ld * 2)) & 7) == 0;
+                        static_cast<const float*>(rows), ld, vec);
   if (dtype == KNN_DTYPE_F16)
     return launch_after(pack_kernel<__half>, grid, kThreads, 0, stream, v, l,
                         static_cast<const __half*>(rows), ld, vec);
