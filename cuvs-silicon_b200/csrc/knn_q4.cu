@@ -114,102 +114,143 @@ __device__ __forceinline__ int64_t list_row(const Q4View& v, const Q4List& l, co
 }
 
 // ------------------------------------------------------------------- pack
-// v / s to the nearest whole number, ties to even, exactly, for s > 0 and
-// quotients below 2^20.  over is 1 / s in fp32, so the product can be one off
-// near a tie; the remainder, exact in one fma (24 + 11 bits and a quotient of
-// 5), tells.
-__device__ __forceinline__ float nearest(float v, float s, float over) {
-  constexpr float kWhole = 12582912.0f;  // 1.5 * 2^23: adding it rounds to whole numbers
-  float n = __fadd_rn(__fmaf_rn(v, over, kWhole), -kWhole);
-  const float left = fmaf(-n, s, v), half = 0.5f * s;
-  if (fabsf(left) >= half) {  // rare
-    const bool odd = (static_cast<int>(n) & 1) != 0;
-    if (fabsf(left) > half || odd) n += copysignf(1.0f, left);
-  }
+// v / s to the nearest whole number, ties to even, exactly, for s > 0.  The
+// quotient in fp32 can fall on a tie that the true one only comes near to; the
+// remainder (exact in one fma where the quotient is below 32) tells.
+__device__ float nearest(float v, float s) {
+  float n = rintf(__fdiv_rn(v, s));
+  if (!(fabsf(n) < 32.0f)) return n;  // clamped by the caller
+  // bf16 scales can be so small that half of one is no longer exact
+  const float up = s < 0x1p-100f ? 0x1p100f : 1.0f;
+  const float left = fmaf(-n, s * up, v * up), half = 0.5f * (s * up);
+  const bool odd = (static_cast<int>(n) & 1) != 0;
+  if (fabsf(left) > half || (fabsf(left) == half && odd)) n += copysignf(1.0f, left);
   return n;
 }
 
+// The codes of 8 values of a group, and the sum of their squares in units of
+// the scale.  Multiplying by 1 / s and adding 1.5 * 2^23 (and 8) leaves the
+// rounded quotient in the lowest bits of the sum; the remainders show whether
+// a quotient came so near to a tie that this may be wrong, and then, or where
+// the scale was rounded so far that codes have to be clamped (it is
+// subnormal), they are computed again with `nearest`.
+template <bool kZeros>
+__device__ __forceinline__ uint32_t codes_of(const float (&a)[8], float s, bool usable, float most,
+                                             float zero, float* square) {
+  const float shift = kZeros ? zero : 8.0f;
+  const float whole = 12582912.0f + shift, over = __fdividef(1.0f, s), half = 0.5f * s;
+  const float cap = 15.0f - shift;
+  float worst = 0.0f, sum = 0.0f;
+  uint32_t packed = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float t = __fmaf_rn(a[e], over, whole);
+    float n = __fadd_rn(t, -whole);
+    worst = fmaxf(worst, fabsf(fmaf(-n, s, a[e])));
+    uint32_t bits = __float_as_uint(t);
+    if (kZeros) {
+      n = fminf(n, cap);
+      bits = __float_as_uint(__fadd_rn(n, whole));
+    }
+    sum = fmaf(n, n, sum);
+    packed += bits << (4 * e);
+  }
+  // each word added was 0x4b400000 + code; of the eight, three reach the end
+  packed -= 0x4b400000u + 0xb4000000u + 0x40000000u;
+  if (!usable || !(worst < half) || !(most * over < (kZeros ? 15.5f : 7.5f)) || s < 0x1p-100f) {
+    packed = 0;
+    sum = 0.0f;
+    for (int e = 0; e < 8; ++e) {
+      float n = 0.0f;
+      if (usable) n = fminf(fmaxf(nearest(a[e], s), -shift), cap);
+      sum = fmaf(n, n, sum);
+      packed |= static_cast<uint32_t>(static_cast<int>(n + shift)) << (4 * e);
+    }
+  }
+  *square = sum;
+  return packed;
+}
+
 // One warp a row; a lane holds 8 neighbouring values of each 256, so that its
-// codes are one word.  HBM bound: values are read once, codes and scales
-// written once.
-template <class T>
+// codes are one word, and asks for 4 such pieces before it works on the first.
+// HBM bound in principle: values are read once, codes and scales written once.
+template <class T, bool kZeros>
 __global__ void __launch_bounds__(kThreads) pack_kernel(Q4View v, Q4List l, const T* x, int64_t ld,
                                                         bool vec) {
+  constexpr int kAhead = 4, kPieces = sizeof(T) / 2;
   __shared__ ListSmem sm;
   wait_for_stream();
   if (l.seqs && !l.status[kStatusApplied]) return;
   if (!open_list(l, sm)) return;  // as the call that made room found it
   const int lane = threadIdx.x & 31;
   const int span = v.group / 8;  // lanes of a group
+  const int dim = static_cast<int>(v.dim), padded = 2 * v.width;
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); t < l.total;
        t += static_cast<int64_t>(gridDim.x) * kWarps) {
     const int64_t row = list_row(v, l, sm, t);
     if (row < 0) continue;
     const T* in = x + t * ld;
+    uint32_t* codes = reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(v.codes) + row * v.width);
+    uint16_t* scales = const_cast<uint16_t*>(v.scales) + row * v.groups;
+    uint8_t* zeros = const_cast<uint8_t*>(v.zeros) + (kZeros ? row * v.groups : 0);
     float norm = 0.0f;
-#pragma unroll 2
-    for (int base = 0; base < 2 * v.width; base += 256) {
-      const int j = base + 8 * lane;
-      float a[8];
-      if (vec && j + 8 <= v.dim) {
-        __align__(16) T h[8];
+    for (int base = 0; base < padded; base += 256 * kAhead) {
+      uint4 raw[kAhead][kPieces];
 #pragma unroll
-        for (int e = 0; e < static_cast<int>(sizeof(T)) / 2; ++e)
-          reinterpret_cast<uint4*>(h)[e] = __ldcs(reinterpret_cast<const uint4*>(in + j) + e);
+      for (int u = 0; u < kAhead; ++u) {
+        const int j = base + 256 * u + 8 * lane;
+        if (vec && j + 8 <= dim) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) a[e] = load_value(h + e);
-      } else {
+          for (int e = 0; e < kPieces; ++e) raw[u][e] = __ldcs(reinterpret_cast<const uint4*>(in + j) + e);
+        } else {
+          __align__(16) T h[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) a[e] = j + e < v.dim ? load_value(in + j + e) : 0.0f;
-      }
-      float low = 0.0f, high = 0.0f;
+          for (int e = 0; e < 8; ++e) h[e] = j + e < dim ? in[j + e] : T(0.0f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        high = max_nan(high, v.zeros ? a[e] : fabsf(a[e]));
-        if (v.zeros) low = max_nan(low, -a[e]);
+          for (int e = 0; e < kPieces; ++e) raw[u][e] = reinterpret_cast<const uint4*>(h)[e];
+        }
       }
-      for (int d = 1; d < span; d <<= 1) {
-        high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, d));
-        if (v.zeros) low = max_nan(low, __shfl_xor_sync(0xffffffffu, low, d));
-      }
-      const float wide = v.zeros ? __fdiv_rn(high + low, 15.0f) : __fdiv_rn(high, 7.0f);
-      uint16_t bits;
-      float s;
-      if (v.scale_bf16) {
-        const __nv_bfloat16 h = __float2bfloat16_rn(wide);
-        bits = __bfloat16_as_ushort(h);
-        s = __bfloat162float(h);
-      } else {
-        const __half h = __float2half_rn(wide);
-        bits = __half_as_ushort(h);
-        s = __half2float(h);
-      }
-      // a scale of 0, or one that is no finite number: all values at the zero point
-      const bool usable = s > 0.0f && s < __int_as_float(0x7f800000);
-      // bf16 scales can be so small that 1 / s overflows: then all of it times 2^100
-      const float up = v.scale_bf16 && s < 0x1p-100f ? 0x1p100f : 1.0f;
-      const float big = s * up, over = __fdiv_rn(1.0f, big);
-      float zero = 8.0f;
-      if (v.zeros) zero = usable ? fminf(fmaxf(nearest(low * up, big, over), 0.0f), 15.0f) : 0.0f;
-      uint32_t packed = 0;
-      float square = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float c = zero;
-        if (usable) c = fminf(fmaxf(nearest(a[e] * up, big, over) + zero, 0.0f), 15.0f);
-        if (j + e >= v.dim) c = 0.0f;
-        const float d = j + e < v.dim ? c - zero : 0.0f;
-        square = fmaf(d, d, square);
-        // 2^23 + c holds c in its lowest bits
-        packed |= (__float_as_uint(c + 8388608.0f) & 15u) << (4 * e);
-      }
-      norm = fmaf(s * s, square, norm);
-      if (j < 2 * v.width)
-        *reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(v.codes) + row * v.width + j / 2) = packed;
-      if (lane % span == 0 && j < v.dim) {
-        const int64_t g = row * v.groups + j / v.group;
-        const_cast<uint16_t*>(v.scales)[g] = bits;
-        if (v.zeros) const_cast<uint8_t*>(v.zeros)[g] = static_cast<uint8_t>(zero);
+      for (int u = 0; u < kAhead; ++u) {
+        if (base + 256 * u >= padded) break;
+        const int j = base + 256 * u + 8 * lane;
+        float a[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] = load_value(reinterpret_cast<const T*>(raw[u]) + e);
+        float low = 0.0f, high = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          high = max_nan(high, kZeros ? a[e] : fabsf(a[e]));
+          if (kZeros) low = max_nan(low, -a[e]);
+        }
+        for (int d = 1; d < span; d <<= 1) {
+          high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, d));
+          if (kZeros) low = max_nan(low, __shfl_xor_sync(0xffffffffu, low, d));
+        }
+        const float wide = kZeros ? __fdiv_rn(high + low, 15.0f) : __fdiv_rn(high, 7.0f);
+        uint16_t bits;
+        float s;
+        if (v.scale_bf16) {
+          const __nv_bfloat16 h = __float2bfloat16_rn(wide);
+          bits = __bfloat16_as_ushort(h);
+          s = __bfloat162float(h);
+        } else {
+          const __half h = __float2half_rn(wide);
+          bits = __half_as_ushort(h);
+          s = __half2float(h);
+        }
+        // a scale of 0, or one that is no finite number: all values at the zero point
+        const bool usable = s > 0.0f && s < __int_as_float(0x7f800000);
+        float zero = 8.0f, square;
+        if (kZeros) zero = usable ? fminf(nearest(low, s), 15.0f) : 0.0f;
+        const uint32_t packed = codes_of<kZeros>(a, s, usable, kZeros ? low : high, zero, &square);
+        // a scale that is no finite number makes the norm NaN, as the values are
+        norm = fmaf(s * s, square, norm);
+        if (j < padded) codes[j >> 3] = packed;
+        if ((lane & (span - 1)) == 0 && j < dim) {
+          scales[j >> v.group_shift] = bits;
+          if (kZeros) zeros[j >> v.group_shift] = static_cast<uint8_t>(zero);
+        }
       }
     }
     if (v.norms) {
@@ -230,32 +271,31 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Q4View v, Q4List l, floa
       atomicCAS(&l.status[kStatusError], 0, KNN_PAGES_BAD_COUNT);
     return;
   }
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, dim = static_cast<int>(v.dim);
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); t < l.total;
        t += static_cast<int64_t>(gridDim.x) * kWarps) {
     const int64_t row = list_row(v, l, sm, t);
-    const uint8_t* codes = v.codes + (row < 0 ? 0 : row) * v.width;
+    const int64_t from = row < 0 ? 0 : row;
+    const uint8_t* codes = v.codes + from * v.width;
+    float* to = out + t * ld;
 #pragma unroll 4
-    for (int j = 4 * lane; j < v.dim; j += 128) {
-      const uint32_t packed = *reinterpret_cast<const uint16_t*>(codes + j / 2);
-      const int g = j / v.group;
-      float s = __int_as_float(0x7fc00000);  // no page: NaN
-      int z = 8;
-      if (row >= 0) {
-        s = scale_of(v, row, g);
-        z = zero_of(v, row, g);
-      }
+    for (int j = 4 * lane; j < dim; j += 128) {
+      const uint32_t packed = *reinterpret_cast<const uint16_t*>(codes + (j >> 1));
+      const int g = j >> v.group_shift;
+      float s = scale_of(v, from, g);
+      if (row < 0) s = __int_as_float(0x7fc00000);  // no page: NaN
+      // 2^23 + code less 2^23 + zero
+      const float z = -(8388608.0f + static_cast<float>(zero_of(v, from, g)));
       float a[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        a[e] = static_cast<float>(static_cast<int>((packed >> (4 * e)) & 15) - z) * s;
-      float* o = out + t * ld + j;
-      if (vec && j + 4 <= v.dim) {
-        __stcs(reinterpret_cast<float4*>(o), make_float4(a[0], a[1], a[2], a[3]));
+        a[e] = __fadd_rn(__uint_as_float(((packed >> (4 * e)) & 15u) | 0x4b000000u), z) * s;
+      if (vec && j + 4 <= dim) {
+        __stcs(reinterpret_cast<float4*>(to + j), make_float4(a[0], a[1], a[2], a[3]));
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (j + e < v.dim) o[e] = a[e];
+          if (j + e < dim) to[j + e] = a[e];
       }
     }
   }
@@ -1084,7 +1124,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
 #pragma unroll 4
     for (int j = 8 * lane; j < v.dim; j += 256) {
       const uint32_t packed = *reinterpret_cast<const uint32_t*>(v.codes + row * v.width + j / 2);
-      const int g = j / v.group;
+      const int g = j >> v.group_shift;
       const float s = scale_of(v, row, g);
       const int z = zero_of(v, row, g);
       float qv[8];
@@ -1234,13 +1274,14 @@ cudaError_t launch_q4_pack(const Q4View& v, const Q4List& l, const void* rows, i
   const uintptr_t bits = reinterpret_cast<uintptr_t>(rows);
   const bool vec = ((bits | (ld * (dtype == KNN_DTYPE_F32 ? 4 : 2))) & 15) == 0;
   if (dtype == KNN_DTYPE_F32)
-    return launch_after(pack_kernel<float>, grid, kThreads, 0, stream, v, l,
-                        static_cast<const float*>(rows), ld, vec);
+    return launch_after(v.zeros ? pack_kernel<float, true> : pack_kernel<float, false>, grid,
+                        kThreads, 0, stream, v, l, static_cast<const float*>(rows), ld, vec);
   if (dtype == KNN_DTYPE_F16)
-    return launch_after(pack_kernel<__half>, grid, kThreads, 0, stream, v, l,
-                        static_cast<const __half*>(rows), ld, vec);
-  return launch_after(pack_kernel<__nv_bfloat16>, grid, kThreads, 0, stream, v, l,
-                      static_cast<const __nv_bfloat16*>(rows), ld, vec);
+    return launch_after(v.zeros ? pack_kernel<__half, true> : pack_kernel<__half, false>, grid,
+                        kThreads, 0, stream, v, l, static_cast<const __half*>(rows), ld, vec);
+  return launch_after(v.zeros ? pack_kernel<__nv_bfloat16, true> : pack_kernel<__nv_bfloat16, false>,
+                      grid, kThreads, 0, stream, v, l, static_cast<const __nv_bfloat16*>(rows), ld,
+                      vec);
 }
 
 cudaError_t launch_q4_read(const Q4View& v, const Q4List& l, float* out, int64_t ld,

@@ -13,6 +13,7 @@ struct Q4View {
   const float* norms;      // [rows], |row|^2, or nullptr
   int64_t dim;
   int32_t group, groups;
+  int32_t group_shift;  // group = 1 << group_shift
   int32_t width;  // bytes of a row's codes, 16 * ceil(dim / 32)
   int32_t scale_bf16;
   Places places;

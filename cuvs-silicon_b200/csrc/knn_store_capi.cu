@@ -111,6 +111,7 @@ knn::Q4View view_of(const knn_q4_rows& q) {
   v.norms = q.norms;
   v.dim = q.dim;
   v.group = q.group;
+  v.group_shift = q.group == 32 ? 5 : q.group == 64 ? 6 : 7;
   v.groups = static_cast<int32_t>((q.dim + q.group - 1) / q.group);
   v.width = static_cast<int32_t>(knn_q4_row_bytes(q.dim));
   v.scale_bf16 = q.scale_dtype == KNN_DTYPE_BF16;

@@ -365,6 +365,23 @@ def test_pack_ties_and_odd_groups(torch, engine):
         assert torch.isnan(rows.norms).tolist() == [False, False, not zero_points, True]
 
 
+def test_pack_small_and_large_scales(torch, engine):
+    """Scales among the subnormal numbers of fp16 and bf16 (codes have to be clamped
+    there) and near bf16's largest."""
+    v = randn(torch, 3, 200, 128)
+    size = 2.0 ** torch.linspace(-30, -16, 200, dtype=torch.float64, device="cuda")
+    cases = [((v.double() * size[:, None]).float(), torch.float16)]
+    for power in (-128, -124, -100, -98, 118, 124):
+        cases.append(((v.double() * 2.0 ** power).float(), torch.bfloat16))
+    for x, scale in cases:
+        for zero_points in (False, True):
+            rows = engine.q4_pack(x, 32, zero_points, scale)
+            codes, scales, zeros, values = plain_pack(torch, x, 32, zero_points, scale)
+            assert torch.equal(rows.scales, scales)
+            assert torch.equal(unpack(torch, rows.codes, 128).double(), codes)
+            assert torch.equal(rows.read().double(), values.float().double())
+
+
 def test_pack_strided_rows(torch, engine):
     wide = randn(torch, 3, 40, 211)
     for dtype in (torch.float32, torch.float16, torch.bfloat16):
