@@ -898,8 +898,10 @@ constexpr int kCandCap = 4096;
 
 constexpr int kBins = 2048;
 constexpr int kMinimaHeld = 32;  // minima that a thread keeps in registers
+constexpr int kQueryHeld = 4096;  // values of the query that are kept in shared memory
 
 struct SelectSmem {
+  float query[kQueryHeld];  // zeros behind the last value
   uint64_t cand[kCandCap];
   uint64_t final_key[kMaxCandidates];
   uint32_t final_row[kMaxCandidates];
@@ -909,6 +911,7 @@ struct SelectSmem {
   uint32_t count, groups;
   uint64_t prefix;
   int64_t rank;
+  int64_t inside;  // values in the bin
 };
 
 // Adds one to the bin of each thread that has one (bin < kBins).  Keys share
@@ -918,8 +921,8 @@ __device__ __forceinline__ void count_bin(SelectSmem& sm, uint32_t bin) {
   if (bin < kBins && (threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(&sm.hist[bin], __popc(same));
 }
 
-// The bin that the value of rank `rank` falls in, and (in sm.rank) its rank
-// there.  All threads; the bins are cleared for the next count.
+// The bin that the value of rank `rank` falls in, (in sm.rank) its rank there
+// and (in sm.inside) how many there are.  All threads; the bins are cleared for the next count.
 __device__ uint32_t find_bin(SelectSmem& sm, int64_t rank) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int kPer = kBins / kSelectThreads;
@@ -951,6 +954,7 @@ __device__ uint32_t find_bin(SelectSmem& sm, int64_t rank) {
     while (left >= static_cast<int64_t>(h[j])) left -= h[j++];
     sm.prefix = static_cast<uint64_t>(kPer * threadIdx.x + j);
     sm.rank = left;
+    sm.inside = h[j];
   }
   __syncthreads();
   return static_cast<uint32_t>(sm.prefix);
@@ -979,13 +983,26 @@ __device__ uint64_t nth(int64_t n, int64_t rank, SelectSmem& sm, Load load) {
   return prefix;
 }
 
-// A bound that at least rank + 1 of the minima lie at or below, and hardly
-// more: the value of that rank with its last 10 bits set (two counts of 11
-// bits).  Up to 32 minima a thread are read once and kept.
-__device__ uint32_t minima_bound(const uint32_t* minima, int64_t groups, int64_t rank,
+// A bound that at least `wanted` of the minima lie at or below, and hardly
+// more: the range of the minima is cut into 2048 equal bins of their ordered
+// form, the bin of the wanted rank again, until few enough lie at or below its
+// end.  Equal bins of the range that there is, not of a number's bits: minima
+// share those, and atomics on one bin run one after another.  Up to 32 minima
+// a thread are read once and kept.
+__device__ uint32_t minima_bound(const uint32_t* minima, int64_t groups, int wanted,
                                  SelectSmem& sm) {
   uint32_t held[kMinimaHeld];
   const bool keep = groups <= kMinimaHeld * kSelectThreads;
+  auto each = [&](auto&& f) {
+    if (keep) {
+#pragma unroll
+      for (int j = 0; j < kMinimaHeld; ++j)
+        if (static_cast<int64_t>(j) * kSelectThreads < groups) f(held[j]);
+    } else {
+#pragma unroll 4
+      for (int64_t i = threadIdx.x; i < groups; i += kSelectThreads) f(minima[i]);
+    }
+  };
   if (keep) {
 #pragma unroll
     for (int j = 0; j < kMinimaHeld; ++j) {
@@ -993,30 +1010,43 @@ __device__ uint32_t minima_bound(const uint32_t* minima, int64_t groups, int64_t
       held[j] = i < groups ? minima[i] : kNoKey;
     }
   }
-  uint32_t prefix = 0;
-#pragma unroll 1
-  for (int pass = 0; pass < 2; ++pass) {
-    const int shift = pass ? 10 : 21;
-    auto count = [&](uint32_t x, bool in) {
-      in = in && (pass == 0 || (x >> 21) == (prefix >> 21));
-      count_bin(sm, in ? (x >> shift) & 2047u : static_cast<uint32_t>(kBins));
-    };
-    if (keep) {
-#pragma unroll
-      for (int j = 0; j < kMinimaHeld; ++j)
-        if (static_cast<int64_t>(j) * kSelectThreads < groups)
-          count(held[j], static_cast<int64_t>(j) * kSelectThreads + threadIdx.x < groups);
-    } else {
-#pragma unroll 4
-      for (int64_t base = 0; base < groups; base += kSelectThreads) {
-        const int64_t i = base + threadIdx.x;
-        count(i < groups ? minima[i] : kNoKey, i < groups);
-      }
-    }
-    prefix |= find_bin(sm, rank) << shift;
-    rank = sm.rank;
+  uint32_t low = kNoKey, high = 0;
+  each([&](uint32_t x) {
+    if (x != kNoKey) low = min(low, x), high = max(high, x);
+  });
+  low = __reduce_min_sync(0xffffffffu, low);
+  high = __reduce_max_sync(0xffffffffu, high);
+  if (threadIdx.x == 0) sm.count = kNoKey, sm.groups = 0;
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) {
+    atomicMin(&sm.count, low);
+    atomicMax(&sm.groups, high);
   }
-  return prefix | 1023u;
+  __syncthreads();
+  low = sm.count, high = sm.groups;
+  if (low > high) return kNoKey - 1;  // no keys at all
+  int64_t rank = wanted - 1;          // counted from low
+  int64_t below = 0;                  // minima below low
+  while (true) {
+    // bins of 2^shift, 2048 of which reach over the range
+    const int bits = 32 - __clz(high - low);
+    const int shift = bits > 11 ? bits - 11 : 0;
+    each([&](uint32_t x) {
+      if (x != kNoKey && x >= low && x <= high) atomicAdd(&sm.hist[(x - low) >> shift], 1u);
+    });
+    if (threadIdx.x == 0) sm.rank = -1;
+    const uint32_t bin = find_bin(sm, rank);
+    if (sm.rank < 0) return high;  // fewer keys than wanted
+    const uint32_t first = low + (bin << shift);
+    const uint32_t last = min(high, first + ((1u << shift) - 1u));
+    const int64_t inside = sm.inside;
+    below += rank - sm.rank;
+    if (shift == 0 || below + inside <= wanted + wanted / 2 + 32) return last;
+    rank = sm.rank;
+    low = first;
+    high = last;
+    __syncthreads();
+  }
 }
 
 // Sorts sm.cand[0 .. n) ascending, n a power of two.
@@ -1062,8 +1092,11 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
   const int wanted = k + kMoreCandidates;
   uint32_t tau = kNoKey - 1;
   for (int i = threadIdx.x; i < kBins; i += kSelectThreads) sm.hist[i] = 0;
+  for (int j = threadIdx.x; j < kQueryHeld && j < ((v.dim + 7) & ~7ll); j += kSelectThreads)
+    sm.query[j] = j < v.dim ? load_value(x + b * ldx + j) : 0.0f;
   __syncthreads();
-  if (groups > wanted) tau = min(minima_bound(minima, groups, wanted - 1, sm), kNoKey - 1);
+  if (groups > wanted) tau = min(minima_bound(minima, groups, wanted, sm), kNoKey - 1);
+  __syncthreads();
   if (threadIdx.x == 0) sm.count = sm.groups = 0;
   __syncthreads();
   for (int64_t g = threadIdx.x; g < groups; g += kSelectThreads)
@@ -1114,28 +1147,42 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
     __syncthreads();
     have = min(static_cast<int>(sm.count), wanted);
   }
-  // distances in 64 bits, a warp to a candidate
-  const int lane = threadIdx.x & 31;
+  // distances in 64 bits, a warp to a candidate; its lanes look its rows up at once
+  constexpr int kSelectWarps = kSelectThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const T* q = x + b * ldx;
-  for (int e = threadIdx.x >> 5; e < have; e += kSelectThreads / 32) {
-    const uint32_t i = static_cast<uint32_t>(sm.cand[e]);
-    const int64_t row = v.places.at(r.seq, i);
+  const int mine = have > warp ? (have - warp + kSelectWarps - 1) / kSelectWarps : 0;
+  uint32_t my_index = 0;
+  int32_t my_row = 0;
+  if (lane < mine) {
+    my_index = static_cast<uint32_t>(sm.cand[warp + kSelectWarps * lane]);
+    my_row = static_cast<int32_t>(v.places.at(r.seq, my_index));
+  }
+  for (int c = 0; c < mine; ++c) {
+    const int e = warp + kSelectWarps * c;
+    const uint32_t i = __shfl_sync(0xffffffffu, my_index, c);
+    const int64_t row = __shfl_sync(0xffffffffu, my_row, c);
     double sum = 0.0;
 #pragma unroll 4
     for (int j = 8 * lane; j < v.dim; j += 256) {
-      const uint32_t packed = *reinterpret_cast<const uint32_t*>(v.codes + row * v.width + j / 2);
+      const uint32_t packed = *reinterpret_cast<const uint32_t*>(v.codes + row * v.width + (j >> 1));
       const int g = j >> v.group_shift;
       const float s = scale_of(v, row, g);
       const int z = zero_of(v, row, g);
       float qv[8];
+      if (j + 8 <= kQueryHeld) {
+        *reinterpret_cast<float4*>(qv) = *reinterpret_cast<const float4*>(sm.query + j);
+        *reinterpret_cast<float4*>(qv + 4) = *reinterpret_cast<const float4*>(sm.query + j + 4);
+      } else {
 #pragma unroll
-      for (int c = 0; c < 8; ++c) qv[c] = j + c < v.dim ? load_value(q + j + c) : 0.0f;
+        for (int f = 0; f < 8; ++f) qv[f] = j + f < v.dim ? load_value(q + j + f) : 0.0f;
+      }
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const int code = static_cast<int>((packed >> (4 * c)) & 15);
+      for (int f = 0; f < 8; ++f) {
+        const int code = static_cast<int>((packed >> (4 * f)) & 15);
         // exact: 5 bits times 11; codes behind the last value count for nothing
-        const double value = j + c < v.dim ? static_cast<float>(code - z) * s : 0.0f;
-        const double term = static_cast<double>(qv[c]);
+        const double value = j + f < v.dim ? static_cast<float>(code - z) * s : 0.0f;
+        const double term = static_cast<double>(qv[f]);
         if (mode == kKeyL2) sum = fma(term - value, term - value, sum);
         else sum = fma(-term, value, sum);
       }
