@@ -320,7 +320,8 @@ struct Q4Out {
   int dtype;
   int64_t ld;
   int mode;
-  uint32_t* minima;  // [vectors][tiles of 32 rows]: smallest key, or nullptr
+  uint32_t* minima;  // [vectors][minima_ld]: smallest key of each tile of 32 rows, or nullptr
+  int64_t minima_ld;
 };
 
 // Stores a product, or makes it a key, which it stores and returns.
@@ -844,7 +845,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1)
               least = min(least, __shfl_xor_sync(0xffffffffu, least, d));
-            if (g == 0 && mine_too) o.minima[b * p.tiles + first / kTileRows4] = least;
+            if (g == 0 && mine_too) o.minima[b * o.minima_ld + first / kTileRows4] = least;
           }
         }
     } else {
@@ -879,7 +880,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         }
         if (o.minima) {
           least = __reduce_min_sync(0xffffffffu, least);
-          if (lane == 0) o.minima[b * p.tiles + tile] = least;
+          if (lane == 0) o.minima[b * o.minima_ld + tile] = least;
         }
       }
       __syncthreads();
@@ -895,14 +896,15 @@ constexpr int kMoreCandidates = 16;  // scored again beyond the k asked for
 constexpr int kMaxCandidates = KNN_MAX_K + kMoreCandidates;
 constexpr int kGroupCap = 1024;
 constexpr int kCandCap = 4096;
+constexpr int kRankCap = 512;  // candidates that are ranked by counting, not sorted
 
 constexpr int kBins = 2048;
-constexpr int kMinimaHeld = 32;  // minima that a thread keeps in registers
 constexpr int kQueryHeld = 4096;  // values of the query that are kept in shared memory
 
 struct SelectSmem {
-  float query[kQueryHeld];  // zeros behind the last value
+  double query[kQueryHeld];  // zeros behind the last value
   uint64_t cand[kCandCap];
+  uint32_t pick[kMaxCandidates];  // rows to score again
   uint64_t final_key[kMaxCandidates];
   uint32_t final_row[kMaxCandidates];
   uint32_t hist[kBins];
@@ -987,29 +989,19 @@ __device__ uint64_t nth(int64_t n, int64_t rank, SelectSmem& sm, Load load) {
 // more: the range of the minima is cut into 2048 equal bins of their ordered
 // form, the bin of the wanted rank again, until few enough lie at or below its
 // end.  Equal bins of the range that there is, not of a number's bits: minima
-// share those, and atomics on one bin run one after another.  Up to 32 minima
-// a thread are read once and kept.
+// share those, and atomics on one bin run one after another.
 __device__ uint32_t minima_bound(const uint32_t* minima, int64_t groups, int wanted,
                                  SelectSmem& sm) {
-  uint32_t held[kMinimaHeld];
-  const bool keep = groups <= kMinimaHeld * kSelectThreads;
   auto each = [&](auto&& f) {
-    if (keep) {
-#pragma unroll
-      for (int j = 0; j < kMinimaHeld; ++j)
-        if (static_cast<int64_t>(j) * kSelectThreads < groups) f(held[j]);
-    } else {
 #pragma unroll 4
-      for (int64_t i = threadIdx.x; i < groups; i += kSelectThreads) f(minima[i]);
+    for (int64_t i = 4 * threadIdx.x; i < groups; i += 4 * kSelectThreads) {
+      const uint4 u = *reinterpret_cast<const uint4*>(minima + i);
+      f(u.x);
+      if (i + 1 < groups) f(u.y);
+      if (i + 2 < groups) f(u.z);
+      if (i + 3 < groups) f(u.w);
     }
   };
-  if (keep) {
-#pragma unroll
-    for (int j = 0; j < kMinimaHeld; ++j) {
-      const int64_t i = static_cast<int64_t>(j) * kSelectThreads + threadIdx.x;
-      held[j] = i < groups ? minima[i] : kNoKey;
-    }
-  }
   uint32_t low = kNoKey, high = 0;
   each([&](uint32_t x) {
     if (x != kNoKey) low = min(low, x), high = max(high, x);
@@ -1088,22 +1080,27 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
   int64_t n = r.count;
   if (r.length) n = *r.length < n ? *r.length : n;
   keys += b * ld;
-  minima += b * groups;
+  minima += b * ((groups + 3) / 4 * 4);  // 16-byte aligned
   const int wanted = k + kMoreCandidates;
   uint32_t tau = kNoKey - 1;
   for (int i = threadIdx.x; i < kBins; i += kSelectThreads) sm.hist[i] = 0;
   for (int j = threadIdx.x; j < kQueryHeld && j < ((v.dim + 7) & ~7ll); j += kSelectThreads)
-    sm.query[j] = j < v.dim ? load_value(x + b * ldx + j) : 0.0f;
+    sm.query[j] = j < v.dim ? static_cast<double>(load_value(x + b * ldx + j)) : 0.0;
   __syncthreads();
   if (groups > wanted) tau = min(minima_bound(minima, groups, wanted, sm), kNoKey - 1);
   __syncthreads();
   if (threadIdx.x == 0) sm.count = sm.groups = 0;
   __syncthreads();
-  for (int64_t g = threadIdx.x; g < groups; g += kSelectThreads)
-    if (minima[g] <= tau) {
-      const uint32_t at = atomicAdd(&sm.groups, 1u);
-      if (at < kGroupCap) sm.group[at] = static_cast<int32_t>(g);
-    }
+  for (int64_t g = 4 * threadIdx.x; g < groups; g += 4 * kSelectThreads) {
+    const uint4 u = *reinterpret_cast<const uint4*>(minima + g);
+    const uint32_t least[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (g + j < groups && least[j] <= tau) {
+        const uint32_t at = atomicAdd(&sm.groups, 1u);
+        if (at < kGroupCap) sm.group[at] = static_cast<int32_t>(g + j);
+      }
+  }
   __syncthreads();
   const uint32_t listed = sm.groups;
   if (listed <= kGroupCap) {
@@ -1117,16 +1114,32 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
     }
     __syncthreads();
   }
+  constexpr int kSelectWarps = kSelectThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int have;
   if (listed <= kGroupCap && sm.count <= kCandCap) {
     const int count = static_cast<int>(sm.count);
-    int size = 2;
-    while (size < count) size <<= 1;
-    if (count > wanted) {
+    have = min(count, wanted);
+    if (count <= wanted) {
+      for (int e = threadIdx.x; e < count; e += kSelectThreads)
+        sm.pick[e] = static_cast<uint32_t>(sm.cand[e]);
+    } else if (count <= kRankCap) {
+      // the place of each among all, a warp to a candidate
+      for (int e = warp; e < count; e += kSelectWarps) {
+        const uint64_t c = sm.cand[e];
+        int before = 0;
+        for (int o = lane; o < count; o += 32) before += sm.cand[o] < c;
+        before = __reduce_add_sync(0xffffffffu, before);
+        if (lane == 0 && before < wanted) sm.pick[before] = static_cast<uint32_t>(c);
+      }
+    } else {
+      int size = 2;
+      while (size < count) size <<= 1;
       for (int e = count + threadIdx.x; e < size; e += kSelectThreads) sm.cand[e] = ~0ull;
       sort_candidates(sm, size);
+      for (int e = threadIdx.x; e < have; e += kSelectThreads)
+        sm.pick[e] = static_cast<uint32_t>(sm.cand[e]);
     }
-    have = min(count, wanted);
   } else {
     // many equal keys: the row of rank wanted - 1 by (key, index), over all rows
     auto load = [&](int64_t i) {
@@ -1141,21 +1154,20 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
       const uint64_t c = load(i);
       if (c <= last && (c >> 32) != kNoKey) {
         const uint32_t at = atomicAdd(&sm.count, 1u);
-        if (at < kCandCap) sm.cand[at] = c;  // at most `wanted`
+        if (at < kMaxCandidates) sm.pick[at] = static_cast<uint32_t>(i);  // at most `wanted`
       }
     }
     __syncthreads();
     have = min(static_cast<int>(sm.count), wanted);
   }
+  __syncthreads();
   // distances in 64 bits, a warp to a candidate; its lanes look its rows up at once
-  constexpr int kSelectWarps = kSelectThreads / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const T* q = x + b * ldx;
   const int mine = have > warp ? (have - warp + kSelectWarps - 1) / kSelectWarps : 0;
   uint32_t my_index = 0;
   int32_t my_row = 0;
   if (lane < mine) {
-    my_index = static_cast<uint32_t>(sm.cand[warp + kSelectWarps * lane]);
+    my_index = sm.pick[warp + kSelectWarps * lane];
     my_row = static_cast<int32_t>(v.places.at(r.seq, my_index));
   }
   for (int c = 0; c < mine; ++c) {
@@ -1169,22 +1181,28 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
       const int g = j >> v.group_shift;
       const float s = scale_of(v, row, g);
       const int z = zero_of(v, row, g);
-      float qv[8];
+      double qv[8];
       if (j + 8 <= kQueryHeld) {
-        *reinterpret_cast<float4*>(qv) = *reinterpret_cast<const float4*>(sm.query + j);
-        *reinterpret_cast<float4*>(qv + 4) = *reinterpret_cast<const float4*>(sm.query + j + 4);
+#pragma unroll
+        for (int f = 0; f < 8; f += 2)
+          *reinterpret_cast<double2*>(qv + f) = *reinterpret_cast<const double2*>(sm.query + j + f);
       } else {
 #pragma unroll
-        for (int f = 0; f < 8; ++f) qv[f] = j + f < v.dim ? load_value(q + j + f) : 0.0f;
+        for (int f = 0; f < 8; ++f)
+          qv[f] = j + f < v.dim ? static_cast<double>(load_value(q + j + f)) : 0.0;
       }
+      // 2^52 + code less 2^52 + zero: no conversion, which runs at a quarter of
+      // the rate; what lies behind the last value counts for nothing
+      const double s64 = s, minus = -(4503599627370496.0 + z);
 #pragma unroll
       for (int f = 0; f < 8; ++f) {
-        const int code = static_cast<int>((packed >> (4 * f)) & 15);
-        // exact: 5 bits times 11; codes behind the last value count for nothing
-        const double value = j + f < v.dim ? static_cast<float>(code - z) * s : 0.0f;
-        const double term = static_cast<double>(qv[f]);
-        if (mode == kKeyL2) sum = fma(term - value, term - value, sum);
-        else sum = fma(-term, value, sum);
+        const double code = __hiloint2double(0x43300000, (packed >> (4 * f)) & 15) + minus;
+        if (mode == kKeyL2) {
+          const double off = fma(-s64, code, qv[f]);
+          if (j + f < v.dim) sum = fma(off, off, sum);
+        } else {
+          sum = fma(-qv[f], s64 * code, sum);
+        }
       }
     }
 #pragma unroll
@@ -1197,13 +1215,14 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
     }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < have; e += kSelectThreads) {
+  for (int e = warp; e < have; e += kSelectWarps) {
     const uint64_t key = sm.final_key[e];
     const uint32_t row = sm.final_row[e];
     int rank = 0;
-    for (int o = 0; o < have; ++o)
+    for (int o = lane; o < have; o += 32)
       rank += sm.final_key[o] < key || (sm.final_key[o] == key && sm.final_row[o] < row);
-    if (rank < k) {
+    rank = __reduce_add_sync(0xffffffffu, rank);
+    if (lane == 0 && rank < k) {
       const uint64_t u = (key >> 63) ? key & 0x7fffffffffffffffull : ~key;
       const double d = __longlong_as_double(static_cast<long long>(u));
       neighbors[b * k + rank] = row;
@@ -1299,6 +1318,7 @@ cudaError_t products_any(const Q4View& v, const Q4Range& r, const void* x, int d
 }
 
 int64_t group_count(int64_t count) { return (count + kGroupRows - 1) / kGroupRows; }
+int64_t minima_ld(int64_t count) { return (group_count(count) + 3) / 4 * 4; }
 
 template <class T>
 cudaError_t select(const Q4View& v, const Q4Range& r, const void* x, int64_t batch, int64_t ldx,
@@ -1343,7 +1363,7 @@ cudaError_t launch_q4_products(const Q4View& v, const Q4Range& r, const void* x,
                                cudaStream_t stream) {
   const int64_t size = dtype == KNN_DTYPE_F32 ? 4 : 2, out_size = out_dtype == KNN_DTYPE_F32 ? 4 : 2;
   for (int64_t b = 0; b < batch; b += kQ4SearchBatch) {
-    const Q4Out o = {static_cast<char*>(out) + b * ldo * out_size, out_dtype, ldo, kStore, nullptr};
+    const Q4Out o = {static_cast<char*>(out) + b * ldo * out_size, out_dtype, ldo, kStore, nullptr, 0};
     if (cudaError_t e = products_any(
             v, r, static_cast<const char*>(x) + b * ldx * size, dtype,
             static_cast<int>(std::min<int64_t>(kQ4SearchBatch, batch - b)), ldx, o, stream))
@@ -1353,7 +1373,7 @@ cudaError_t launch_q4_products(const Q4View& v, const Q4Range& r, const void* x,
 }
 
 int64_t q4_search_bytes(int64_t count) {
-  return kQ4SearchBatch * 4 * (group_count(count) * (kGroupRows + 1));
+  return kQ4SearchBatch * 4 * (group_count(count) * kGroupRows + minima_ld(count));
 }
 
 cudaError_t launch_q4_search(const Q4View& v, const Q4Range& r, const void* x, int dtype,
@@ -1368,7 +1388,7 @@ cudaError_t launch_q4_search(const Q4View& v, const Q4Range& r, const void* x, i
     const int64_t m = std::min<int64_t>(kQ4SearchBatch, batch - b);
     const void* q = static_cast<const char*>(x) + b * ldx * size;
     if (r.count > 0) {
-      const Q4Out o = {keys, KNN_DTYPE_F32, ld, mode, minima};
+      const Q4Out o = {keys, KNN_DTYPE_F32, ld, mode, minima, minima_ld(r.count)};
       if (cudaError_t e = products_any(v, r, q, dtype, static_cast<int>(m), ldx, o, stream)) return e;
     }
     cudaError_t e;
