@@ -893,7 +893,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
 constexpr int kGroupRows = kTileRows4;  // rows whose smallest key is kept
 constexpr int kSelectThreads = 1024;
 constexpr int kMoreCandidates = 16;  // scored again beyond the k asked for
-constexpr int kMaxCandidates = KNN_MAX_K + kMoreCandidates;
+constexpr int kMaxCandidates = KNN_MAX_K + 2 * kMoreCandidates;
 constexpr int kGroupCap = 1024;
 constexpr int kCandCap = 4096;
 constexpr int kRankCap = 512;  // candidates that are ranked by counting, not sorted
@@ -1096,6 +1096,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
   __syncthreads();
   if (threadIdx.x == 0) sm.count = sm.groups = 0;
   __syncthreads();
+#pragma unroll 4
   for (int64_t g = 4 * threadIdx.x; g < groups; g += 4 * kSelectThreads) {
     const uint4 u = *reinterpret_cast<const uint4*>(minima + g);
     const uint32_t least[4] = {u.x, u.y, u.z, u.w};
@@ -1109,6 +1110,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
   __syncthreads();
   const uint32_t listed = sm.groups;
   if (listed <= kGroupCap) {
+#pragma unroll 4
     for (uint32_t e = threadIdx.x; e < listed * kGroupRows; e += kSelectThreads) {
       const int64_t i = static_cast<int64_t>(sm.group[e / kGroupRows]) * kGroupRows + e % kGroupRows;
       const uint32_t key = i < n ? ordered(keys[i]) : kNoKey;
@@ -1125,7 +1127,8 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
   if (listed <= kGroupCap && sm.count <= kCandCap) {
     const int count = static_cast<int>(sm.count);
     have = min(count, wanted);
-    if (count <= wanted) {
+    if (count <= wanted + kMoreCandidates) {  // a few more do no harm
+      have = count;
       for (int e = threadIdx.x; e < count; e += kSelectThreads)
         sm.pick[e] = static_cast<uint32_t>(sm.cand[e]);
     } else if (count <= kRankCap) {
@@ -1175,65 +1178,87 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
     my_index = sm.pick[warp + kSelectWarps * lane];
     my_row = static_cast<int32_t>(v.places.at(r.seq, my_index));
   }
+  constexpr int kAhead = 4;  // pieces of 256 codes that are asked for at once
+  const int dim = static_cast<int>(v.dim);
   for (int c = 0; c < mine; ++c) {
-    const int e = warp + kSelectWarps * c;
-    const uint32_t i = __shfl_sync(0xffffffffu, my_index, c);
     const int64_t row = __shfl_sync(0xffffffffu, my_row, c);
-    double sum = 0.0;
-#pragma unroll 4
-    for (int j = 8 * lane; j < v.dim; j += 256) {
-      const uint32_t packed = *reinterpret_cast<const uint32_t*>(v.codes + row * v.width + (j >> 1));
-      const int g = j >> v.group_shift;
-      const float s = scale_of(v, row, g);
-      const int z = zero_of(v, row, g);
-      double qv[8];
-      if (j + 8 <= kQueryHeld) {
+    const uint32_t i = __shfl_sync(0xffffffffu, my_index, c);
+    const uint8_t* codes = v.codes + row * v.width;
+    const uint16_t* scales = v.scales + row * v.groups;
+    const uint8_t* zeros = v.zeros ? v.zeros + row * v.groups : nullptr;
+    double sum[2] = {0.0, 0.0};
+    for (int base = 0; base < dim; base += 256 * kAhead) {
+      uint32_t packed[kAhead], bits[kAhead], zero[kAhead];
 #pragma unroll
-        for (int f = 0; f < 4; ++f) {
-          const double2 pair = sm.query[f][j >> 3];
-          qv[2 * f] = pair.x;
-          qv[2 * f + 1] = pair.y;
+      for (int u = 0; u < kAhead; ++u) {
+        const int j = base + 256 * u + 8 * lane;
+        packed[u] = 0, bits[u] = 0, zero[u] = 8;
+        if (j < dim) {
+          packed[u] = *reinterpret_cast<const uint32_t*>(codes + (j >> 1));
+          bits[u] = scales[j >> v.group_shift];
+          if (zeros) zero[u] = zeros[j >> v.group_shift] & 15u;
         }
-      } else {
-#pragma unroll
-        for (int f = 0; f < 8; ++f)
-          qv[f] = j + f < v.dim ? static_cast<double>(load_value(q + j + f)) : 0.0;
       }
-      // 2^52 + code less 2^52 + zero: no conversion, which runs at a quarter of
-      // the rate; what lies behind the last value counts for nothing
-      const double s64 = s, minus = -(4503599627370496.0 + z);
 #pragma unroll
-      for (int f = 0; f < 8; ++f) {
-        const double code = __hiloint2double(0x43300000, (packed >> (4 * f)) & 15) + minus;
-        if (mode == kKeyL2) {
-          const double off = fma(-s64, code, qv[f]);
-          if (j + f < v.dim) sum = fma(off, off, sum);
-        } else {
-          sum = fma(-qv[f], s64 * code, sum);
+      for (int u = 0; u < kAhead; ++u) {
+        const int j = base + 256 * u + 8 * lane;
+        if (base + 256 * u >= dim) break;
+        const double s = v.scale_bf16
+                             ? __uint_as_float(bits[u] << 16)
+                             : __half2float(__ushort_as_half(static_cast<unsigned short>(bits[u])));
+        // 2^52 + code less 2^52 + zero: no conversion, which runs at a quarter
+        // of the rate
+        const double minus = -__hiloint2double(0x43300000, static_cast<int>(zero[u]));
+        double part = 0.0;
+#pragma unroll
+        for (int f = 0; f < 8; f += 2) {
+          double2 pair;
+          if (j + 8 <= kQueryHeld) {
+            pair = sm.query[f >> 1][j >> 3];
+          } else {
+            pair.x = j + f < dim ? static_cast<double>(load_value(q + j + f)) : 0.0;
+            pair.y = j + f + 1 < dim ? static_cast<double>(load_value(q + j + f + 1)) : 0.0;
+          }
+          const double x0 = __hiloint2double(0x43300000, (packed[u] >> (4 * f)) & 15) + minus;
+          const double x1 = __hiloint2double(0x43300000, (packed[u] >> (4 * f + 4)) & 15) + minus;
+          if (mode == kKeyL2) {
+            // what lies behind the last value counts for nothing
+            const double d0 = fma(-s, x0, pair.x), d1 = fma(-s, x1, pair.y);
+            if (j + f < dim) sum[0] = fma(d0, d0, sum[0]);
+            if (j + f + 1 < dim) sum[1] = fma(d1, d1, sum[1]);
+          } else if (j + f < dim) {
+            part = fma(pair.x, x0, fma(pair.y, x1, part));
+          }
         }
+        if (mode != kKeyL2 && j < dim) sum[u & 1] = fma(-s, part, sum[u & 1]);
       }
     }
+    double all = sum[0] + sum[1];
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    for (int d = 16; d >= 1; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
     if (lane == 0) {
-      if (sum != sum) sum = __longlong_as_double(0x7ff0000000000000ll);
-      const uint64_t u = static_cast<uint64_t>(__double_as_longlong(sum + 0.0));
-      sm.final_key[e] = (u >> 63) ? ~u : u | 0x8000000000000000ull;
-      sm.final_row[e] = i;
+      if (all != all) all = __longlong_as_double(0x7ff0000000000000ll);
+      const uint64_t u = static_cast<uint64_t>(__double_as_longlong(all + 0.0));
+      sm.final_key[warp + kSelectWarps * c] = (u >> 63) ? ~u : u | 0x8000000000000000ull;
+      sm.final_row[warp + kSelectWarps * c] = i;
     }
   }
   __syncthreads();
-  for (int e = warp; e < have; e += kSelectWarps) {
-    const uint64_t key = sm.final_key[e];
-    const uint32_t row = sm.final_row[e];
+  // the place of each among all, 8 lanes to a candidate
+  for (int base = 0; base < have; base += kSelectThreads / 8) {
+    const int e = base + (threadIdx.x >> 3);
+    const uint64_t key = e < have ? sm.final_key[e] : 0;
+    const uint32_t index = e < have ? sm.final_row[e] : 0;
     int rank = 0;
-    for (int o = lane; o < have; o += 32)
-      rank += sm.final_key[o] < key || (sm.final_key[o] == key && sm.final_row[o] < row);
-    rank = __reduce_add_sync(0xffffffffu, rank);
-    if (lane == 0 && rank < k) {
+#pragma unroll 4
+    for (int o = threadIdx.x & 7; o < have; o += 8)
+      rank += sm.final_key[o] < key || (sm.final_key[o] == key && sm.final_row[o] < index);
+#pragma unroll
+    for (int d = 4; d >= 1; d >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, d);
+    if ((threadIdx.x & 7) == 0 && e < have && rank < k) {
       const uint64_t u = (key >> 63) ? key & 0x7fffffffffffffffull : ~key;
       const double d = __longlong_as_double(static_cast<long long>(u));
-      neighbors[b * k + rank] = row;
+      neighbors[b * k + rank] = index;
       distances[b * k + rank] = static_cast<float>(mode == kKeyL2 ? d : -d);
     }
   }
