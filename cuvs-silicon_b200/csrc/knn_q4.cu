@@ -899,7 +899,7 @@ constexpr int kCandCap = 4096;
 constexpr int kRankCap = 512;  // candidates that are ranked by counting, not sorted
 
 constexpr int kBins = 2048;
-constexpr int kQueryHeld = 4096;  // values of the query that are kept in shared memory
+constexpr int kQueryHeld = 8192;  // values up to which a query is kept in shared memory
 
 struct SelectSmem {
   // values 8 i + 2 f and 8 i + 2 f + 1 in [f][i]: lanes take values 8 apart, and
@@ -1070,11 +1070,10 @@ __device__ void sort_candidates(SelectSmem& sm, int n) {
 // Candidates: with c wanted and tau the c-th smallest of the groups' minima,
 // c rows lie at or below tau, so only keys <= tau are looked at, and they are
 // in the groups whose minimum is <= tau: c groups, unless keys are equal.
-template <class T>
+template <class T, int kMode, bool kWide>
 __global__ void __launch_bounds__(kSelectThreads) select_kernel(
     Q4View v, Q4Range r, const T* x, int64_t ldx, const float* keys, int64_t ld,
-    const uint32_t* minima, int64_t groups, int k, int mode, int64_t* neighbors,
-    float* distances) {
+    const uint32_t* minima, int64_t groups, int k, int64_t* neighbors, float* distances) {
   extern __shared__ __align__(16) uint8_t raw[];
   SelectSmem& sm = *reinterpret_cast<SelectSmem*>(raw);
   wait_for_stream();
@@ -1086,7 +1085,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
   const int wanted = k + kMoreCandidates;
   uint32_t tau = kNoKey - 1;
   for (int i = threadIdx.x; i < kBins; i += kSelectThreads) sm.hist[i] = 0;
-  for (int j = threadIdx.x; j < kQueryHeld && j < ((v.dim + 7) & ~7ll); j += kSelectThreads) {
+  for (int j = threadIdx.x; !kWide && j < ((v.dim + 255) & ~255ll); j += kSelectThreads) {
     const double value = j < v.dim ? static_cast<double>(load_value(x + b * ldx + j)) : 0.0;
     double2& pair = sm.query[(j & 7) >> 1][j >> 3];
     (j & 1 ? pair.y : pair.x) = value;
@@ -1209,28 +1208,34 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
         // 2^52 + code less 2^52 + zero: no conversion, which runs at a quarter
         // of the rate
         const double minus = -__hiloint2double(0x43300000, static_cast<int>(zero[u]));
-        double part = 0.0;
+        // codes behind the last value: at the zero point, so that they count for nothing
+        uint32_t word = packed[u];
+        if (j + 8 > dim) {
+          const uint32_t keep = j < dim ? (1u << (4 * (dim - j))) - 1u : 0u;
+          word = (word & keep) | (zero[u] * 0x11111111u & ~keep);
+        }
+        double part[2] = {0.0, 0.0};
 #pragma unroll
         for (int f = 0; f < 8; f += 2) {
           double2 pair;
-          if (j + 8 <= kQueryHeld) {
+          if constexpr (!kWide) {
             pair = sm.query[f >> 1][j >> 3];
           } else {
             pair.x = j + f < dim ? static_cast<double>(load_value(q + j + f)) : 0.0;
             pair.y = j + f + 1 < dim ? static_cast<double>(load_value(q + j + f + 1)) : 0.0;
           }
-          const double x0 = __hiloint2double(0x43300000, (packed[u] >> (4 * f)) & 15) + minus;
-          const double x1 = __hiloint2double(0x43300000, (packed[u] >> (4 * f + 4)) & 15) + minus;
-          if (mode == kKeyL2) {
-            // what lies behind the last value counts for nothing
+          const double x0 = __hiloint2double(0x43300000, (word >> (4 * f)) & 15) + minus;
+          const double x1 = __hiloint2double(0x43300000, (word >> (4 * f + 4)) & 15) + minus;
+          if constexpr (kMode == kKeyL2) {
             const double d0 = fma(-s, x0, pair.x), d1 = fma(-s, x1, pair.y);
-            if (j + f < dim) sum[0] = fma(d0, d0, sum[0]);
-            if (j + f + 1 < dim) sum[1] = fma(d1, d1, sum[1]);
-          } else if (j + f < dim) {
-            part = fma(pair.x, x0, fma(pair.y, x1, part));
+            sum[0] = fma(d0, d0, sum[0]);
+            sum[1] = fma(d1, d1, sum[1]);
+          } else {
+            part[0] = fma(pair.x, x0, part[0]);
+            part[1] = fma(pair.y, x1, part[1]);
           }
         }
-        if (mode != kKeyL2 && j < dim) sum[u & 1] = fma(-s, part, sum[u & 1]);
+        if constexpr (kMode != kKeyL2) sum[u & 1] = fma(-s, part[0] + part[1], sum[u & 1]);
       }
     }
     double all = sum[0] + sum[1];
@@ -1259,12 +1264,12 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
       const uint64_t u = (key >> 63) ? key & 0x7fffffffffffffffull : ~key;
       const double d = __longlong_as_double(static_cast<long long>(u));
       neighbors[b * k + rank] = index;
-      distances[b * k + rank] = static_cast<float>(mode == kKeyL2 ? d : -d);
+      distances[b * k + rank] = static_cast<float>(kMode == kKeyL2 ? d : -d);
     }
   }
   for (int e = have + threadIdx.x; e < k; e += kSelectThreads) {
     neighbors[b * k + e] = -1;
-    distances[b * k + e] = __int_as_float(mode == kKeyL2 ? 0x7f800000 : 0xff800000);
+    distances[b * k + e] = __int_as_float(kMode == kKeyL2 ? 0x7f800000 : 0xff800000);
   }
 }
 
@@ -1353,16 +1358,27 @@ cudaError_t products_any(const Q4View& v, const Q4Range& r, const void* x, int d
 int64_t group_count(int64_t count) { return (count + kGroupRows - 1) / kGroupRows; }
 int64_t minima_ld(int64_t count) { return (group_count(count) + 3) / 4 * 4; }
 
+template <class T, int kMode, bool kWide>
+cudaError_t select_as(const Q4View& v, const Q4Range& r, const void* x, int64_t batch, int64_t ldx,
+                      const float* keys, int64_t ld, const uint32_t* minima, int k,
+                      int64_t* neighbors, float* distances, cudaStream_t stream) {
+  auto kernel = select_kernel<T, kMode, kWide>;
+  static std::atomic<uint64_t> allowed{0};
+  if (cudaError_t e = allow_smem(kernel, sizeof(SelectSmem), &allowed)) return e;
+  store_count_launches(1);
+  return launch_after(kernel, static_cast<unsigned>(batch), kSelectThreads, sizeof(SelectSmem),
+                      stream, v, r, static_cast<const T*>(x), ldx, keys, ld, minima,
+                      group_count(r.count), k, neighbors, distances);
+}
+
 template <class T>
 cudaError_t select(const Q4View& v, const Q4Range& r, const void* x, int64_t batch, int64_t ldx,
                    const float* keys, int64_t ld, const uint32_t* minima, int k, int mode,
                    int64_t* neighbors, float* distances, cudaStream_t stream) {
-  static std::atomic<uint64_t> allowed{0};
-  if (cudaError_t e = allow_smem(select_kernel<T>, sizeof(SelectSmem), &allowed)) return e;
-  store_count_launches(1);
-  return launch_after(select_kernel<T>, static_cast<unsigned>(batch), kSelectThreads,
-                      sizeof(SelectSmem), stream, v, r, static_cast<const T*>(x), ldx, keys, ld,
-                      minima, group_count(r.count), k, mode, neighbors, distances);
+  const bool wide = v.dim > kQueryHeld;
+  auto f = mode == kKeyL2 ? (wide ? select_as<T, kKeyL2, true> : select_as<T, kKeyL2, false>)
+                          : (wide ? select_as<T, kKeyProduct, true> : select_as<T, kKeyProduct, false>);
+  return f(v, r, x, batch, ldx, keys, ld, minima, k, neighbors, distances, stream);
 }
 
 }  // namespace

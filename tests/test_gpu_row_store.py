@@ -253,6 +253,9 @@ def plain_search(torch, values, q, k, metric):
     (50000, 1024, 1, 1, 128, F16, False, 0, 0),
     (50000, 130, 40, 16, 64, F32, False, 1, 0),
     (140000, 64, 5, 256, 64, F32, False, 1, 128),
+    (600, 9001, 3, 20, 64, F32, True, 0, 0),
+    (600, 8192, 2, 20, 128, F16, False, 1, 16),
+    (1100000, 32, 2, 50, 32, BF16, True, 0, 0),
 ])
 def test_search(torch, engine, n, dim, batch, k, group, x, zeros, metric, page_rows):
     rows, values = random_rows(torch, engine, n + k, n, dim, group, zeros, torch.float16, page_rows)
