@@ -28,8 +28,11 @@ namespace knn {
 
 namespace {
 
-constexpr int kPlanThreads = 1024;
-constexpr int kPlanWarps = kPlanThreads / 32;
+// Threads of a plan kernel.  Small calls are a chain of loads and barriers:
+// 256 threads go through it faster than 1024 (fork of one sequence 9.3 -> 6 us
+// for the plan), which long lists and many pages need.
+constexpr int kFewThreads = 256, kManyThreads = 1024;
+constexpr int64_t kFewList = 1024, kFewPages = 32768;
 constexpr int kMaxList = KNN_PAGES_MAX_LIST;
 constexpr int kMoveThreads = 256;
 constexpr int64_t kMoveChunk = 16384;  // bytes of a page that one CTA moves at a time
@@ -38,14 +41,15 @@ constexpr int kKeepChunk = 128;        // positions of a sequence that one CTA c
 
 // ------------------------------------------------------------ plan kernels
 struct PlanSmem {
-  unsigned long long part[kPlanWarps];
-  unsigned long long total;
+  unsigned long long part[kManyThreads / 32];
   int bad;
 };
 
 // Exclusive prefix sum over the block; *total gets the sum.
+template <int kThreads>
 __device__ unsigned long long block_exclusive(unsigned long long v, PlanSmem& sm,
                                               unsigned long long* total) {
+  constexpr int kWarps = kThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   unsigned long long inc = v;
 #pragma unroll
@@ -53,22 +57,18 @@ __device__ unsigned long long block_exclusive(unsigned long long v, PlanSmem& sm
     const unsigned long long o = __shfl_up_sync(0xffffffffu, inc, d);
     if (lane >= d) inc += o;
   }
-  __syncthreads();  // the last call's readers are done with part and total
+  __syncthreads();  // the last call's readers are done with part
   if (lane == 31) sm.part[warp] = inc;
   __syncthreads();
-  if (warp == 0) {
-    unsigned long long w = sm.part[lane], s = w;
+  // every warp adds the warps' sums up for itself
+  unsigned long long w = lane < kWarps ? sm.part[lane] : 0, s = w;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const unsigned long long o = __shfl_up_sync(0xffffffffu, s, d);
-      if (lane >= d) s += o;
-    }
-    sm.part[lane] = s - w;
-    if (lane == 31) sm.total = s;
+  for (int d = 1; d < kWarps; d <<= 1) {
+    const unsigned long long o = __shfl_up_sync(0xffffffffu, s, d);
+    if (lane >= d) s += o;
   }
-  __syncthreads();
-  *total = sm.total;
-  return sm.part[warp] + inc - v;
+  *total = __shfl_sync(0xffffffffu, s, kWarps - 1);
+  return __shfl_sync(0xffffffffu, s - w, warp) + inc - v;
 }
 
 // Sets a bit of a shared bitmap; false if it was set already.
@@ -90,21 +90,15 @@ __device__ bool plan_goes_on(const knn_pages& p, PlanSmem& sm) {
   return bad == 0;
 }
 
-// Gives out the `need` lowest-numbered free pages: give(rank, page) for ranks
-// 0 .. need - 1 in order of the page numbers.  Returns how many there were.
-// The block reads the counts in tiles of 16 a thread, four 16-byte loads
-// that are each coalesced; the four runs of a tile are ranked by one prefix
-// sum over four 16-bit fields (a run counts at most 4096).
-template <class Give>
-__device__ int take_free(const knn_pages& p, int need, PlanSmem& sm, Give give) {
-  constexpr int kRun = 4 * kPlanThreads;
-  int given = 0;
-  for (int64_t base = 0; base < p.pages && given < need; base += 4 * kRun) {
-    int4 r[4];
-    unsigned long long count = 0;
+// The counts of references of a tile of 16 pages a thread: four 16-byte loads
+// that are each coalesced.
+template <int kThreads>
+struct RefsTile {
+  int4 r[4];
+  __device__ __forceinline__ void load(const knn_pages& p, int64_t base) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int64_t i = base + j * kRun + 4 * threadIdx.x;
+      const int64_t i = base + j * 4 * kThreads + 4 * threadIdx.x;
       if (i + 4 <= p.pages && (reinterpret_cast<uintptr_t>(p.refs) & 15) == 0) {
         r[j] = *reinterpret_cast<const int4*>(p.refs + i);
       } else {
@@ -113,22 +107,44 @@ __device__ int take_free(const knn_pages& p, int need, PlanSmem& sm, Give give) 
         r[j].z = i + 2 < p.pages ? p.refs[i + 2] : 1;
         r[j].w = i + 3 < p.pages ? p.refs[i + 3] : 1;
       }
-      const int c = (r[j].x == 0) + (r[j].y == 0) + (r[j].z == 0) + (r[j].w == 0);
+    }
+  }
+};
+
+// Gives out the `need` lowest-numbered free pages: give(rank, page) for ranks
+// 0 .. need - 1 in order of the page numbers.  Returns how many there were.
+// `tile` holds the first tile, asked for when the kernel began; the next is
+// asked for while one is ranked.  The four runs of a tile are ranked by one
+// prefix sum over four 16-bit fields (a run counts at most 4096).
+template <int kThreads, class Give>
+__device__ int take_free(const knn_pages& p, int need, PlanSmem& sm, RefsTile<kThreads>& tile,
+                         Give give) {
+  constexpr int kRun = 4 * kThreads;
+  int given = 0;
+  for (int64_t base = 0; base < p.pages && given < need; base += 4 * kRun) {
+    const RefsTile<kThreads> now = tile;
+    tile.load(p, base + 4 * kRun);
+    unsigned long long count = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int4& r = now.r[j];
+      const int c = (r.x == 0) + (r.y == 0) + (r.z == 0) + (r.w == 0);
       count |= static_cast<unsigned long long>(c) << (16 * j);
     }
     unsigned long long total;
-    const unsigned long long before = block_exclusive(count, sm, &total);
+    const unsigned long long before = block_exclusive<kThreads>(count, sm, &total);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+      const int4& r = now.r[j];
       const int64_t i = base + j * kRun + 4 * threadIdx.x;
       int rank = given + static_cast<int>((before >> (16 * j)) & 0xffff);
-      if (r[j].x == 0 && rank < need) give(rank, static_cast<int32_t>(i));
-      rank += r[j].x == 0;
-      if (r[j].y == 0 && rank < need) give(rank, static_cast<int32_t>(i + 1));
-      rank += r[j].y == 0;
-      if (r[j].z == 0 && rank < need) give(rank, static_cast<int32_t>(i + 2));
-      rank += r[j].z == 0;
-      if (r[j].w == 0 && rank < need) give(rank, static_cast<int32_t>(i + 3));
+      if (r.x == 0 && rank < need) give(rank, static_cast<int32_t>(i));
+      rank += r.x == 0;
+      if (r.y == 0 && rank < need) give(rank, static_cast<int32_t>(i + 1));
+      rank += r.y == 0;
+      if (r.z == 0 && rank < need) give(rank, static_cast<int32_t>(i + 2));
+      rank += r.z == 0;
+      if (r.w == 0 && rank < need) give(rank, static_cast<int32_t>(i + 3));
       given += static_cast<int>((total >> (16 * j)) & 0xffff);
     }
   }
@@ -151,7 +167,8 @@ __device__ __forceinline__ int64_t pages_for(int64_t rows, int page_rows) {
 }
 
 // grow: counts[i] more rows for sequence seqs[i].
-__global__ void __launch_bounds__(kPlanThreads) grow_kernel(knn_pages p, const int32_t* seqs,
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads) grow_kernel(knn_pages p, const int32_t* seqs,
                                                             const int32_t* counts, int n,
                                                             int64_t wanted) {
   extern __shared__ uint32_t dyn[];
@@ -160,10 +177,12 @@ __global__ void __launch_bounds__(kPlanThreads) grow_kernel(knn_pages p, const i
   uint32_t* seen = dyn + n + 1;                      // bitmap of the sequences
   const int64_t words = (p.sequences + 31) / 32;
   if (threadIdx.x == 0) sm.bad = 0;
-  for (int64_t i = threadIdx.x; i < words; i += kPlanThreads) seen[i] = 0;
+  for (int64_t i = threadIdx.x; i < words; i += kThreads) seen[i] = 0;
   wait_for_stream();
+  RefsTile<kThreads> tile;
+  tile.load(p, 0);
   __syncthreads();
-  constexpr int kPer = kMaxList / kPlanThreads;
+  constexpr int kPer = (kThreads == kFewThreads ? kFewList : kMaxList) / kThreads;
   unsigned long long fresh[kPer], mine = 0, rows_sum = 0;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
@@ -184,8 +203,8 @@ __global__ void __launch_bounds__(kPlanThreads) grow_kernel(knn_pages p, const i
     mine += fresh[j];
   }
   unsigned long long need = 0, rows_total = 0;
-  unsigned long long before = block_exclusive(mine, sm, &need);
-  block_exclusive(rows_sum, sm, &rows_total);
+  unsigned long long before = block_exclusive<kThreads>(mine, sm, &need);
+  block_exclusive<kThreads>(rows_sum, sm, &rows_total);
   if (wanted >= 0 && rows_total != static_cast<unsigned long long>(wanted))
     raise(sm, KNN_PAGES_BAD_COUNT);
   if (need > static_cast<unsigned long long>(p.pages)) raise(sm, KNN_PAGES_NONE_FREE);
@@ -204,13 +223,13 @@ __global__ void __launch_bounds__(kPlanThreads) grow_kernel(knn_pages p, const i
       return p.table + s * p.columns + pages_for(p.rows[s], p.page_rows) + (rank - first[i]);
     };
     const int want = static_cast<int>(need);
-    const int got = take_free(p, want, sm, [&](int rank, int32_t page) {
+    const int got = take_free<kThreads>(p, want, sm, tile, [&](int rank, int32_t page) {
       *entry(rank) = page;
       p.refs[page] = 1;
     });
     __syncthreads();
     if (got < want) {  // too few: give them back
-      for (int rank = threadIdx.x; rank < got; rank += kPlanThreads) {
+      for (int rank = threadIdx.x; rank < got; rank += kThreads) {
         int32_t* e = entry(rank);
         p.refs[*e] = 0;
         *e = -1;
@@ -219,7 +238,7 @@ __global__ void __launch_bounds__(kPlanThreads) grow_kernel(knn_pages p, const i
     }
   }
   if (!plan_goes_on(p, sm)) return;
-  for (int i = threadIdx.x; i < n; i += kPlanThreads) p.rows[seqs[i]] += counts[i];
+  for (int i = threadIdx.x; i < n; i += kThreads) p.rows[seqs[i]] += counts[i];
 }
 
 // ------------------------------------------------------------------- free
@@ -280,7 +299,8 @@ __device__ __forceinline__ void block_copy(uint8_t* to, const uint8_t* from, int
 }
 
 // copy, plan: every index in range, no target twice, no target a source.
-__global__ void __launch_bounds__(kPlanThreads) copy_plan_kernel(knn_pages p,
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads) copy_plan_kernel(knn_pages p,
                                                                  const int32_t* sources,
                                                                  const int32_t* targets,
                                                                  int64_t n) {
@@ -288,16 +308,16 @@ __global__ void __launch_bounds__(kPlanThreads) copy_plan_kernel(knn_pages p,
   __shared__ PlanSmem sm;
   const int64_t words = (p.pages + 31) / 32;
   if (threadIdx.x == 0) sm.bad = 0;
-  for (int64_t i = threadIdx.x; i < words; i += kPlanThreads) dyn[i] = 0;
+  for (int64_t i = threadIdx.x; i < words; i += kThreads) dyn[i] = 0;
   wait_for_stream();
   __syncthreads();
-  for (int64_t i = threadIdx.x; i < n; i += kPlanThreads) {
+  for (int64_t i = threadIdx.x; i < n; i += kThreads) {
     const int32_t t = targets[i];
     if (t < 0 || t >= p.pages) raise(sm, KNN_PAGES_OUT_OF_RANGE);
     else if (!mark(dyn, t)) raise(sm, KNN_PAGES_LISTED_TWICE);
   }
   __syncthreads();
-  for (int64_t i = threadIdx.x; i < n; i += kPlanThreads) {
+  for (int64_t i = threadIdx.x; i < n; i += kThreads) {
     const int32_t s = sources[i];
     if (s < 0 || s >= p.pages) raise(sm, KNN_PAGES_OUT_OF_RANGE);
     else if ((dyn[s >> 5] >> (s & 31)) & 1) raise(sm, KNN_PAGES_LISTED_TWICE);
@@ -332,7 +352,8 @@ __global__ void __launch_bounds__(kMoveThreads) copy_kernel(knn_pages p, const i
 // -------------------------------------------------------------------- fork
 // fork, plan: the children's lengths, and a fresh page for each child whose
 // parent's last page is not full.
-__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(knn_pages p,
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads) fork_plan_kernel(knn_pages p,
                                                                  const int32_t* parents,
                                                                  const int32_t* children, int n) {
   extern __shared__ uint32_t dyn[];
@@ -342,10 +363,12 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(knn_pages p,
   uint32_t* seen = dyn + 2 * n;
   const int64_t words = (p.sequences + 31) / 32;
   if (threadIdx.x == 0) sm.bad = 0;
-  for (int64_t i = threadIdx.x; i < words; i += kPlanThreads) seen[i] = 0;
+  for (int64_t i = threadIdx.x; i < words; i += kThreads) seen[i] = 0;
   wait_for_stream();
+  RefsTile<kThreads> tile;
+  tile.load(p, 0);
   __syncthreads();
-  constexpr int kPer = kMaxList / kPlanThreads;
+  constexpr int kPer = (kThreads == kFewThreads ? kFewList : kMaxList) / kThreads;
   unsigned long long mine = 0;
   bool part[kPer];
 #pragma unroll
@@ -366,7 +389,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(knn_pages p,
     mine += part[j];
   }
   unsigned long long need = 0;
-  int before = static_cast<int>(block_exclusive(mine, sm, &need));
+  int before = static_cast<int>(block_exclusive<kThreads>(mine, sm, &need));
 #pragma unroll
   for (int j = 0; j < kPer; ++j)
     if (part[j]) who[before++] = threadIdx.x * kPer + j;
@@ -377,13 +400,13 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(knn_pages p,
       return p.table + children[i] * p.columns + length[i] / p.page_rows;
     };
     const int want = static_cast<int>(need);
-    const int got = take_free(p, want, sm, [&](int rank, int32_t page) {
+    const int got = take_free<kThreads>(p, want, sm, tile, [&](int rank, int32_t page) {
       *entry(rank) = page;
       p.refs[page] = 1;
     });
     __syncthreads();
     if (got < want) {
-      for (int rank = threadIdx.x; rank < got; rank += kPlanThreads) {
+      for (int rank = threadIdx.x; rank < got; rank += kThreads) {
         int32_t* e = entry(rank);
         p.refs[*e] = 0;
         *e = -1;
@@ -392,7 +415,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(knn_pages p,
     }
   }
   if (!plan_goes_on(p, sm)) return;
-  for (int i = threadIdx.x; i < n; i += kPlanThreads) p.rows[children[i]] = length[i];
+  for (int i = threadIdx.x; i < n; i += kThreads) p.rows[children[i]] = length[i];
 }
 
 // fork, move: full pages are shared (table entry, one more reference), the
@@ -466,7 +489,8 @@ __global__ void __launch_bounds__(kKeepChunk) compact_count_kernel(
   if (threadIdx.x == 0) w.kept[i * w.chunks + chunk] = count;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(knn_pages p,
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads) compact_plan_kernel(knn_pages p,
                                                                     const int32_t* sources,
                                                                     const int32_t* targets, int n,
                                                                     int64_t keep_columns,
@@ -478,10 +502,12 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(knn_pages p,
   const int64_t words = (p.sequences + 31) / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) sm.bad = 0;
-  for (int64_t i = threadIdx.x; i < words; i += kPlanThreads) seen[i] = 0;
+  for (int64_t i = threadIdx.x; i < words; i += kThreads) seen[i] = 0;
   wait_for_stream();
+  RefsTile<kThreads> tile;
+  tile.load(p, 0);
   // rows kept before each chunk, a warp to a sequence
-  for (int64_t i = warp; i < n; i += kPlanWarps) {
+  for (int64_t i = warp; i < n; i += (kThreads / 32)) {
     int32_t* kept = w.kept + i * w.chunks;
     int sum = 0;
     for (int64_t base = 0; base < w.chunks; base += 32) {
@@ -499,7 +525,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(knn_pages p,
     if (lane == 0) w.total[i] = sum;
   }
   __syncthreads();
-  constexpr int kPer = kMaxList / kPlanThreads;
+  constexpr int kPer = (kThreads == kFewThreads ? kFewList : kMaxList) / kThreads;
   unsigned long long fresh[kPer], mine = 0;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
@@ -517,7 +543,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(knn_pages p,
     mine += fresh[j];
   }
   unsigned long long need = 0;
-  unsigned long long before = block_exclusive(mine, sm, &need);
+  unsigned long long before = block_exclusive<kThreads>(mine, sm, &need);
   if (need > static_cast<unsigned long long>(p.pages)) raise(sm, KNN_PAGES_NONE_FREE);
   __syncthreads();
   if (sm.bad == 0) {
@@ -533,28 +559,44 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(knn_pages p,
       return w.fresh + i * p.columns + (rank - first[i]);
     };
     const int want = static_cast<int>(need);
-    const int got = take_free(p, want, sm, [&](int rank, int32_t page) {
+    const int got = take_free<kThreads>(p, want, sm, tile, [&](int rank, int32_t page) {
       *entry(rank) = page;
       p.refs[page] = 1;
     });
     __syncthreads();
     if (got < want) {
-      for (int rank = threadIdx.x; rank < got; rank += kPlanThreads) p.refs[*entry(rank)] = 0;
+      for (int rank = threadIdx.x; rank < got; rank += kThreads) p.refs[*entry(rank)] = 0;
       raise(sm, KNN_PAGES_NONE_FREE);
     }
   }
   plan_goes_on(p, sm);
 }
 
-// The kept rows of a chunk go to their places, piece by piece.
+// The kept rows of a chunk go to their places, piece by piece, four of a
+// thread's under way at once.
 template <class T>
 __device__ __forceinline__ void gather_rows(T* pool, const int64_t* from, const int64_t* to,
                                             int kept, int64_t row_bytes) {
   const uint32_t pieces = static_cast<uint32_t>(row_bytes / sizeof(T));
   const uint32_t total = pieces * kept;
-  for (uint32_t i = threadIdx.x; i < total; i += kMoveThreads) {
-    const uint32_t r = i / pieces, c = i - r * pieces;
-    pool[to[r] * pieces + c] = pool[from[r] * pieces + c];
+  // i / pieces by the reciprocal: it is at most `pieces` / 2^32 too large, and
+  // i below kKeepChunk * pieces, so exact up to 4096 pieces
+  const uint32_t over = 0xffffffffu / pieces + 1;
+  const bool exact = pieces > 1 && pieces <= 4096;
+  for (uint32_t i = threadIdx.x; i < total; i += 4 * kMoveThreads) {
+    T v[4];
+    int64_t at[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t o = i + j * kMoveThreads;
+      if (o >= total) continue;
+      const uint32_t r = exact ? __umulhi(o, over) : o / pieces, c = o - r * pieces;
+      at[j] = to[r] * pieces + c;
+      v[j] = pool[from[r] * pieces + c];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j * kMoveThreads < total) pool[at[j]] = v[j];
   }
 }
 
@@ -629,6 +671,20 @@ __global__ void __launch_bounds__(kMoveThreads) compact_commit_kernel(knn_pages 
 
 constexpr int kPlanSmem = 200 * 1024;  // at most: a bitmap of 2^20 bits and lists of 2 x 4096
 
+// Launches a plan kernel in its form for few or for many entries and pages.
+template <class... P, class... A>
+cudaError_t launch_plan(void (*few)(P...), void (*many)(P...), int64_t n, const knn_pages& p,
+                        size_t smem, cudaStream_t stream, A&&... args) {
+  const bool small = n <= kFewList && p.pages <= kFewPages;
+  if (smem > 40 * 1024) {
+    if (cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(small ? few : many),
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, kPlanSmem))
+      return e;
+  }
+  return launch_after(small ? few : many, 1, small ? kFewThreads : kManyThreads, smem, stream,
+                      args...);
+}
+
 int64_t move_chunks(const knn_pages& p) {
   int64_t chunks = 0;
   for (int k = 0; k < p.n_pools; ++k)
@@ -645,12 +701,9 @@ unsigned move_grid(int64_t items) {
 cudaError_t launch_pages_grow(const knn_pages& p, const int32_t* seqs, const int32_t* counts,
                               int64_t n, int64_t total, cudaStream_t stream) {
   const size_t smem = 4 * (n + 1 + (p.sequences + 31) / 32);
-  static std::atomic<uint64_t> allowed{0};
-  if (smem > 40 * 1024)
-    if (cudaError_t e = allow_smem(grow_kernel, kPlanSmem, &allowed)) return e;
   store_count_launches(1);
-  return launch_after(grow_kernel, 1, kPlanThreads, smem, stream, p, seqs, counts,
-                      static_cast<int>(n), total);
+  return launch_plan(grow_kernel<kFewThreads>, grow_kernel<kManyThreads>, n, p, smem, stream, p,
+                     seqs, counts, static_cast<int>(n), total);
 }
 
 cudaError_t launch_pages_free(const knn_pages& p, const int32_t* seqs, int64_t n,
@@ -663,12 +716,9 @@ cudaError_t launch_pages_free(const knn_pages& p, const int32_t* seqs, int64_t n
 cudaError_t launch_pages_copy(const knn_pages& p, const int32_t* sources, const int32_t* targets,
                               int64_t n, cudaStream_t stream) {
   const size_t smem = 4 * ((p.pages + 31) / 32);
-  static std::atomic<uint64_t> allowed{0};
-  if (smem > 40 * 1024)
-    if (cudaError_t e = allow_smem(copy_plan_kernel, kPlanSmem, &allowed)) return e;
   store_count_launches(2);
-  if (cudaError_t e = launch_after(copy_plan_kernel, 1, kPlanThreads, smem, stream, p, sources,
-                                   targets, n))
+  if (cudaError_t e = launch_plan(copy_plan_kernel<kFewThreads>, copy_plan_kernel<kManyThreads>, n,
+                                  p, smem, stream, p, sources, targets, n))
     return e;
   const int64_t chunks = move_chunks(p);
   return launch_after(copy_kernel, move_grid(n * chunks), kMoveThreads, 0, stream, p, sources,
@@ -678,12 +728,9 @@ cudaError_t launch_pages_copy(const knn_pages& p, const int32_t* sources, const 
 cudaError_t launch_pages_fork(const knn_pages& p, const int32_t* parents, const int32_t* children,
                               int64_t n, cudaStream_t stream) {
   const size_t smem = 4 * (2 * n + (p.sequences + 31) / 32);
-  static std::atomic<uint64_t> allowed{0};
-  if (smem > 40 * 1024)
-    if (cudaError_t e = allow_smem(fork_plan_kernel, kPlanSmem, &allowed)) return e;
   store_count_launches(2);
-  if (cudaError_t e = launch_after(fork_plan_kernel, 1, kPlanThreads, smem, stream, p, parents,
-                                   children, static_cast<int>(n)))
+  if (cudaError_t e = launch_plan(fork_plan_kernel<kFewThreads>, fork_plan_kernel<kManyThreads>, n,
+                                  p, smem, stream, p, parents, children, static_cast<int>(n)))
     return e;
   const int64_t shares = (p.columns + kShareChunk - 1) / kShareChunk, chunks = move_chunks(p);
   return launch_after(fork_kernel, move_grid(n * (shares + chunks)), kMoveThreads, 0, stream, p,
@@ -705,16 +752,14 @@ cudaError_t launch_pages_compact(const knn_pages& p, const int32_t* sources,
   w.total = w.kept + n * w.chunks;
   w.fresh = w.total + n;
   const size_t smem = 4 * (n + (p.sequences + 31) / 32);
-  static std::atomic<uint64_t> allowed{0};
-  if (smem > 40 * 1024)
-    if (cudaError_t e = allow_smem(compact_plan_kernel, kPlanSmem, &allowed)) return e;
   store_count_launches(4);
   const unsigned grid = static_cast<unsigned>(n * w.chunks);
   if (cudaError_t e = launch_after(compact_count_kernel, grid, kKeepChunk, 0, stream, p, sources,
                                    keep, keep_columns, keep_stride, w))
     return e;
-  if (cudaError_t e = launch_after(compact_plan_kernel, 1, kPlanThreads, smem, stream, p, sources,
-                                   targets, static_cast<int>(n), keep_columns, w))
+  if (cudaError_t e = launch_plan(compact_plan_kernel<kFewThreads>,
+                                  compact_plan_kernel<kManyThreads>, n, p, smem, stream, p, sources,
+                                  targets, static_cast<int>(n), keep_columns, w))
     return e;
   if (cudaError_t e = launch_after(compact_kernel, grid, kMoveThreads, 0, stream, p, sources, keep,
                                    keep_stride, w))

@@ -390,10 +390,10 @@ def _on_device(name, t, device, dtype=None, shape=None, dense=True):
 
 
 def _list(name, t, device):
-    import torch
-
-    _on_device(name, t, device, torch.int32)
-    if t.dim() != 1:
+    # one test where nothing is wrong: this is most of what a small call costs here
+    if not (getattr(t, "is_cuda", False) and t.dtype is _torch().int32 and t.dim() == 1
+            and t.device == device and t.is_contiguous()):
+        _on_device(name, t, device, _torch().int32)
         raise ValueError(f"{name} must be a list of int32")
     return t
 
@@ -405,26 +405,46 @@ def _two_lists(names, a, b, device):
         raise ValueError(f"{names[0]} and {names[1]} differ in length")
 
 
-def _stream(device) -> int:
-    import torch
+_torch_module = None
+_raw_stream = None
 
-    return torch.cuda.current_stream(device).cuda_stream
+
+def _torch():
+    """torch, which only the row store needs."""
+    global _torch_module, _raw_stream
+    if _torch_module is None:
+        import torch
+
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _torch_module = torch
+    return _torch_module
+
+
+def _stream(device) -> int:
+    """The device's current torch stream."""
+    if _raw_stream is not None:
+        return _raw_stream(device.index)
+    return _torch().cuda.current_stream(device).cuda_stream
 
 
 def _rows_of(name, t, device, dim):
     """A matrix of vectors (or one vector) of floats whose values lie side by side."""
-    import torch
-
-    codes = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
+    torch = _torch()
     _on_device(name, t, device, dense=False)
-    if t.dtype not in codes:
-        raise ValueError(f"{name} of {t.dtype}: not float32, float16 or bfloat16")
-    if t.dim() not in (1, 2) or t.shape[-1] != dim:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, not (n, {dim})")
-    if (dim > 1 and t.stride(-1) != 1) or (t.dim() == 2 and t.shape[0] > 1 and t.stride(0) < dim):
+    dtype = t.dtype
+    code = (DTYPE_F32 if dtype is torch.float32 else DTYPE_F16 if dtype is torch.float16 else
+            DTYPE_BF16 if dtype is torch.bfloat16 else None)
+    if code is None:
+        raise ValueError(f"{name} of {dtype}: not float32, float16 or bfloat16")
+    shape = t.shape
+    flat = len(shape) == 1
+    if (not flat and len(shape) != 2) or shape[-1] != dim:
+        raise ValueError(f"{name} has shape {tuple(shape)}, not (n, {dim})")
+    n = 1 if flat else shape[0]
+    ld = dim if n == 1 else t.stride(0)
+    if (dim > 1 and t.stride(-1) != 1) or ld < dim and n > 0:
         raise ValueError(f"{name}: the values of a row must lie side by side, rows apart")
-    n = t.shape[0] if t.dim() == 2 else 1
-    return n, (t.stride(0) if t.dim() == 2 and n > 1 else dim), codes[t.dtype]
+    return n, ld, code
 
 
 class Pages:
@@ -443,8 +463,7 @@ class Pages:
     """
 
     def __init__(self, table, rows, refs, pools):
-        import torch
-
+        torch = _torch()
         _on_device("table", table, None, torch.int32)
         device = table.device
         if table.dim() != 2:
@@ -480,8 +499,7 @@ class Pages:
     @classmethod
     def empty(cls, pools, sequences: int, columns: int):
         """A store of empty sequences over the given pools."""
-        import torch
-
+        torch = _torch()
         pools = list(pools)
         if not pools or not getattr(pools[0], "is_cuda", False):
             raise ValueError("pools must be CUDA tensors")
@@ -518,8 +536,7 @@ class Pages:
     def compact(self, sources, targets, keep) -> None:
         """targets[i] (empty, or sources[i] itself) becomes the rows j of
         sources[i] with keep[i, j], in order, in fresh pages."""
-        import torch
-
+        torch = _torch()
         _two_lists(("sources", "targets"), sources, targets, self.device)
         _on_device("keep", keep, self.device, dense=False)
         n = sources.shape[0]
@@ -557,8 +574,7 @@ class Q4Rows:
     """
 
     def __init__(self, codes, scales, dim: int, group: int, zeros=None, norms=None, pages=None):
-        import torch
-
+        torch = _torch()
         _on_device("codes", codes, None, torch.uint8)
         device, lead = codes.device, tuple(codes.shape[:-1])
         if dim < 1 or group not in (32, 64, 128):
@@ -616,8 +632,7 @@ class Q4Rows:
     def read(self, seqs=None, counts=None, total=None, first: int = 0):
         """The values of rows, float32: rows first .. first + total - 1 of dense
         rows, or the last counts[i] rows of seqs[i], ``total`` in all."""
-        import torch
-
+        torch = _torch()
         if self.pages is None:
             if seqs is not None or counts is not None:
                 raise ValueError("dense rows have no sequences")
@@ -640,8 +655,7 @@ class Q4Rows:
         """x [batch, dim] (or one vector) times rows 0 .. count - 1: [batch,
         count] in ``dtype`` (float32 unless given).  In pages: of sequence
         ``seq``, 0 beyond its length."""
-        import torch
-
+        torch = _torch()
         seq, count = self._range(seq, count)
         n, ldx, code = _rows_of("x", x, self.device, self.dim)
         if count < 0 or count > self.n_rows:
@@ -661,8 +675,7 @@ class Q4Rows:
     def search(self, queries, k: int, metric: int = METRIC_L2_EXPANDED, seq=None, count=None):
         """The k nearest rows of each query: (neighbors int64, distances
         float32), as Index.search orders and pads them."""
-        import torch
-
+        torch = _torch()
         seq, count = self._range(seq, count)
         n, ld, code = _rows_of("queries", queries, self.device, self.dim)
         if queries.dim() != 2:
@@ -684,8 +697,7 @@ def q4_pack(rows, group: int = 64, zero_points: bool = False, scale_dtype=None) 
     """Quantises rows [n, dim] (float32, float16 or bfloat16) to 4 bits with a
     scale (float16 unless ``scale_dtype`` says bfloat16), and where asked a
     zero point, for every ``group`` values; see knn_q4_pack in the C header."""
-    import torch
-
+    torch = _torch()
     if getattr(rows, "ndim", 0) != 2 or rows.shape[1] < 1 or group not in (32, 64, 128):
         raise ValueError("rows must be 2-D, in groups of 32, 64 or 128")
     n, dim = rows.shape
