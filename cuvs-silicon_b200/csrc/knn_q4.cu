@@ -262,8 +262,13 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(Q4View v, Q4List l, cons
 }
 
 // ------------------------------------------------------------------- read
+// One warp a row; a lane turns 4 codes of each 128 into 16 bytes, and asks for
+// 8 such pieces before it works on the first.  HBM bound: 4 bytes are written
+// for half a byte that is read.
+template <bool kZeros>
 __global__ void __launch_bounds__(kThreads) read_kernel(Q4View v, Q4List l, float* out, int64_t ld,
                                                         bool vec) {
+  constexpr int kAhead = 8;
   __shared__ ListSmem sm;
   wait_for_stream();
   if (!open_list(l, sm)) {
@@ -271,31 +276,46 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Q4View v, Q4List l, floa
       atomicCAS(&l.status[kStatusError], 0, KNN_PAGES_BAD_COUNT);
     return;
   }
-  const int lane = threadIdx.x & 31, dim = static_cast<int>(v.dim);
+  const int lane = threadIdx.x & 31, dim = static_cast<int>(v.dim), shift = v.group_shift;
+  const bool bf16 = v.scale_bf16;
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); t < l.total;
        t += static_cast<int64_t>(gridDim.x) * kWarps) {
     const int64_t row = list_row(v, l, sm, t);
     const int64_t from = row < 0 ? 0 : row;
     const uint8_t* codes = v.codes + from * v.width;
+    const uint16_t* scales = v.scales + from * v.groups;
+    const uint8_t* zeros = v.zeros + (kZeros ? from * v.groups : 0);
     float* to = out + t * ld;
-#pragma unroll 4
-    for (int j = 4 * lane; j < dim; j += 128) {
-      const uint32_t packed = *reinterpret_cast<const uint16_t*>(codes + (j >> 1));
-      const int g = j >> v.group_shift;
-      float s = scale_of(v, from, g);
-      if (row < 0) s = __int_as_float(0x7fc00000);  // no page: NaN
-      // 2^23 + code less 2^23 + zero
-      const float z = -(8388608.0f + static_cast<float>(zero_of(v, from, g)));
-      float a[4];
+    for (int base = 4 * lane; base < dim; base += 128 * kAhead) {
+      uint32_t packed[kAhead], bits[kAhead], zero[kAhead];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        a[e] = __fadd_rn(__uint_as_float(((packed >> (4 * e)) & 15u) | 0x4b000000u), z) * s;
-      if (vec && j + 4 <= dim) {
-        __stcs(reinterpret_cast<float4*>(to + j), make_float4(a[0], a[1], a[2], a[3]));
-      } else {
+      for (int u = 0; u < kAhead; ++u) {
+        const int j = base + 128 * u;
+        if (j >= dim) continue;
+        packed[u] = *reinterpret_cast<const uint16_t*>(codes + (j >> 1));
+        bits[u] = scales[j >> shift];
+        if (kZeros) zero[u] = zeros[j >> shift] & 15u;
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int j = base + 128 * u;
+        if (j >= dim) continue;
+        float s = __half2float(__ushort_as_half(static_cast<unsigned short>(bits[u])));
+        if (bf16) s = __uint_as_float(bits[u] << 16);
+        if (row < 0) s = __int_as_float(0x7fc00000);  // no page: NaN
+        // 2^23 + code less 2^23 + zero
+        const float z = __uint_as_float(0xcb000000u + (kZeros ? zero[u] : 8u));
+        float a[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (j + e < dim) to[j + e] = a[e];
+          a[e] = __fadd_rn(__uint_as_float(((packed[u] >> (4 * e)) & 15u) | 0x4b000000u), z) * s;
+        if (vec && j + 4 <= dim) {
+          __stcs(reinterpret_cast<float4*>(to + j), make_float4(a[0], a[1], a[2], a[3]));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (j + e < dim) to[j + e] = a[e];
+        }
       }
     }
   }
@@ -1404,7 +1424,8 @@ cudaError_t launch_q4_read(const Q4View& v, const Q4List& l, float* out, int64_t
                            cudaStream_t stream) {
   store_count_launches(1);
   const bool vec = ((reinterpret_cast<uintptr_t>(out) | (ld * 4)) & 15) == 0;
-  return launch_after(read_kernel, row_grid(l.total), kThreads, 0, stream, v, l, out, ld, vec);
+  return launch_after(v.zeros ? read_kernel<true> : read_kernel<false>, row_grid(l.total), kThreads,
+                      0, stream, v, l, out, ld, vec);
 }
 
 cudaError_t launch_q4_products(const Q4View& v, const Q4Range& r, const void* x, int dtype,

@@ -26,13 +26,15 @@ struct Places {
   int64_t columns;
   int64_t pages;
   int32_t page_rows;
+  // Positions are below 2^31, as a store's rows are: 32-bit division.
   __device__ __forceinline__ int64_t at(int64_t seq, int64_t position) const {
     if (!table) return position;
-    const int64_t column = position / page_rows;
+    const uint32_t p = static_cast<uint32_t>(position);
+    const uint32_t column = p / static_cast<uint32_t>(page_rows);
     if (column >= columns) return -1;
     const int32_t page = table[seq * columns + column];
     if (page < 0 || page >= pages) return -1;
-    return static_cast<int64_t>(page) * page_rows + (position - column * page_rows);
+    return static_cast<int64_t>(page) * page_rows + (p - column * page_rows);
   }
 };
 
