@@ -128,6 +128,16 @@ __device__ float nearest(float v, float s) {
   return n;
 }
 
+// a / kBy, rounded as IEEE asks: a product with the rounded reciprocal, and one
+// correction by its exact remainder (Markstein's theorem; it needs the
+// remainder not to underflow).
+template <int kBy>
+__device__ __forceinline__ float divided(float a) {
+  constexpr float kOver = 1.0f / kBy;
+  const float q = a * kOver, fine = fmaf(fmaf(-q, static_cast<float>(kBy), a), kOver, q);
+  return a > 1e-30f && a < 1e38f ? fine : __fdiv_rn(a, static_cast<float>(kBy));
+}
+
 // The codes of 8 values of a group, and the sum of their squares in units of
 // the scale.  Multiplying by 1 / s and adding 1.5 * 2^23 (and 8) leaves the
 // rounded quotient in the lowest bits of the sum; the remainders show whether
@@ -223,11 +233,13 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(Q4View v, Q4List l, cons
           high = max_nan(high, kZeros ? a[e] : fabsf(a[e]));
           if (kZeros) low = max_nan(low, -a[e]);
         }
-        for (int d = 1; d < span; d <<= 1) {
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) {
+          if (d >= span) continue;
           high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, d));
           if (kZeros) low = max_nan(low, __shfl_xor_sync(0xffffffffu, low, d));
         }
-        const float wide = kZeros ? __fdiv_rn(high + low, 15.0f) : __fdiv_rn(high, 7.0f);
+        const float wide = kZeros ? divided<15>(high + low) : divided<7>(high);
         uint16_t bits;
         float s;
         if (v.scale_bf16) {
