@@ -610,17 +610,25 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   // warp finds those of its four rows side by side: as fp32, or with zero
   // points as they are held, below 1024 + zero in fp16.
   auto put_scales = [&](uint32_t* to) {
+    to += lane;
+    if constexpr (kZeros) {
 #pragma unroll
-    for (int j = 0; j < 2 * kGroups; ++j) {
-      const uint32_t bits = (held.s[j >> 1] >> (16 * (j & 1))) & 0xffffu;
-      uint32_t word;
-      if (kZeros) {
-        word = bits | ((held.z[j >> 2] >> (8 * (j & 3))) & 15u) << 16 | 0x64000000u;
-      } else {
-        word = __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(bits))));
-        if (v.scale_bf16) word = bits << 16;
+      for (int j = 0; j < 2 * kGroups; ++j)
+        to[j * kTileRows4] = ((held.s[j >> 1] >> (16 * (j & 1))) & 0xffffu) |
+                             ((held.z[j >> 2] >> (8 * (j & 3))) & 15u) << 16 | 0x64000000u;
+    } else if (v.scale_bf16) {
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j) {
+        to[2 * j * kTileRows4] = held.s[j] << 16;
+        to[(2 * j + 1) * kTileRows4] = held.s[j] & 0xffff0000u;
       }
-      to[j * kTileRows4 + lane] = word;
+    } else {
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j) {
+        const float2 two = __half22float2(*reinterpret_cast<const __half2*>(&held.s[j]));
+        to[2 * j * kTileRows4] = __float_as_uint(two.x);
+        to[(2 * j + 1) * kTileRows4] = __float_as_uint(two.y);
+      }
     }
   };
   // ---- the vectors' scales
