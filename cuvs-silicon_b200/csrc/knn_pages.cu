@@ -265,11 +265,18 @@ __global__ void __launch_bounds__(kMoveThreads) free_kernel(knn_pages p, const i
   if (bad || again) return;
   int64_t used = pages_for(p.rows[s], p.page_rows);
   if (used > p.columns) used = p.columns;
-  for (int64_t c = threadIdx.x; c < used; c += kMoveThreads) {
-    int32_t* e = p.table + s * p.columns + c;
-    const int32_t page = *e;
-    if (page >= 0 && page < p.pages) atomicSub(&p.refs[page], 1);
-    *e = -1;
+  // four entries of a thread's under way at once: a long sequence is a latency
+  int32_t* entries = p.table + s * p.columns;
+  for (int64_t c = threadIdx.x; c < used; c += 4 * kMoveThreads) {
+    int32_t page[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      page[j] = c + j * kMoveThreads < used ? entries[c + j * kMoveThreads] : -1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (page[j] >= 0 && page[j] < p.pages) atomicSub(&p.refs[page[j]], 1);
+      if (c + j * kMoveThreads < used) entries[c + j * kMoveThreads] = -1;
+    }
   }
   __syncthreads();
   if (threadIdx.x == 0) p.rows[s] = 0;
@@ -510,16 +517,25 @@ __global__ void __launch_bounds__(kThreads) compact_plan_kernel(knn_pages p,
   for (int64_t i = warp; i < n; i += (kThreads / 32)) {
     int32_t* kept = w.kept + i * w.chunks;
     int sum = 0;
-    for (int64_t base = 0; base < w.chunks; base += 32) {
-      const int64_t c = base + lane;
-      const int v = c < w.chunks ? kept[c] : 0;
-      int inc = v;
+    for (int64_t base = 0; base < w.chunks; base += 128) {
+      const int64_t c = base + 4 * lane;
+      int v[4], mine = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = c + j < w.chunks ? kept[c + j] : 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mine += v[j];
+      int inc = mine;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int o = __shfl_up_sync(0xffffffffu, inc, d);
         if (lane >= d) inc += o;
       }
-      if (c < w.chunks) kept[c] = sum + inc - v;
+      int before = sum + inc - mine;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (c + j < w.chunks) kept[c + j] = before;
+        before += v[j];
+      }
       sum += __shfl_sync(0xffffffffu, inc, 31);
     }
     if (lane == 0) w.total[i] = sum;

@@ -1462,8 +1462,9 @@ cudaError_t launch_q4_products(const Q4View& v, const Q4Range& r, const void* x,
   return cudaSuccess;
 }
 
-int64_t q4_search_bytes(int64_t count) {
-  return kQ4SearchBatch * 4 * (group_count(count) * kGroupRows + minima_ld(count));
+int64_t q4_search_bytes(int64_t count, int64_t batch) {
+  return std::min<int64_t>(batch, kQ4SearchBatch) * 4 *
+         (group_count(count) * kGroupRows + minima_ld(count));
 }
 
 cudaError_t launch_q4_search(const Q4View& v, const Q4Range& r, const void* x, int dtype,
@@ -1472,7 +1473,8 @@ cudaError_t launch_q4_search(const Q4View& v, const Q4Range& r, const void* x, i
   const int mode = metric == KNN_METRIC_L2_EXPANDED ? kKeyL2 : kKeyProduct;
   const int64_t groups = group_count(r.count), ld = groups * kGroupRows;
   float* keys = static_cast<float*>(workspace);
-  uint32_t* minima = static_cast<uint32_t*>(workspace) + kQ4SearchBatch * ld;
+  uint32_t* minima =
+      static_cast<uint32_t*>(workspace) + std::min<int64_t>(batch, kQ4SearchBatch) * ld;
   const int64_t size = dtype == KNN_DTYPE_F32 ? 4 : 2;
   for (int64_t b = 0; b < batch; b += kQ4SearchBatch) {
     const int64_t m = std::min<int64_t>(kQ4SearchBatch, batch - b);

@@ -49,7 +49,7 @@ cudaError_t launch_q4_products(const Q4View& v, const Q4Range& r, const void* x,
                                cudaStream_t stream);
 // Queries that one pass of a search takes, and its workspace in bytes.
 constexpr int kQ4SearchBatch = 16;
-int64_t q4_search_bytes(int64_t count);
+int64_t q4_search_bytes(int64_t count, int64_t batch);
 cudaError_t launch_q4_search(const Q4View& v, const Q4Range& r, const void* x, int dtype,
                              int64_t batch, int64_t ldx, int k, int metric, int64_t* neighbors,
                              float* distances, void* workspace, cudaStream_t stream);

@@ -313,8 +313,8 @@ int knn_q4_products(const knn_q4_rows* q, int64_t seq, int64_t count, const void
                                       static_cast<cudaStream_t>(stream)));
 }
 
-int64_t knn_q4_search_workspace(int64_t count) {
-  return count < 0 ? -1 : 16 + knn::q4_search_bytes(count);
+int64_t knn_q4_search_workspace(int64_t count, int64_t n_queries) {
+  return count < 0 || n_queries < 0 ? -1 : 16 + knn::q4_search_bytes(count, n_queries);
 }
 
 int knn_q4_search(const knn_q4_rows* q, int64_t seq, int64_t count, const void* queries, int dtype,

@@ -136,7 +136,7 @@ def lib() -> ctypes.CDLL:
         "knn_q4_append": (I, [P, P, P, I64, P, I, I64, I64, P]),
         "knn_q4_read": (I, [P, P, P, I64, I64, I64, P, I64, P]),
         "knn_q4_products": (I, [P, I64, I64, P, I, I64, I64, P, I, I64, P]),
-        "knn_q4_search_workspace": (I64, [I64]),
+        "knn_q4_search_workspace": (I64, [I64, I64]),
         "knn_q4_search": (I, [P, I64, I64, P, I, I64, I64, I64, I, P, P, P, P]),
         "knn_dispatch_count": (ctypes.c_uint64, []),
         "knn_reset_dispatch_count": (None, []),
@@ -686,7 +686,7 @@ class Q4Rows:
             raise ValueError(f"{count} of {self.n_rows} rows")
         neighbors = torch.empty((n, k), dtype=torch.int64, device=self.device)
         distances = torch.empty((n, k), dtype=torch.float32, device=self.device)
-        work = torch.empty(lib().knn_q4_search_workspace(count), dtype=torch.uint8, device=self.device)
+        work = torch.empty(lib().knn_q4_search_workspace(count, n), dtype=torch.uint8, device=self.device)
         _check(lib().knn_q4_search(self._ref, seq, count, queries.data_ptr(), code, n, ld, k, metric,
                                    neighbors.data_ptr(), distances.data_ptr(), work.data_ptr(),
                                    _stream(self.device)))

@@ -510,7 +510,7 @@ int knn_q4_products(const knn_q4_rows* q4, int64_t seq, int64_t count, const voi
  * neighbour.  L2 needs the norms.  workspace: knn_q4_search_workspace bytes
  * of device memory (16-byte aligned), which this call alone uses until it is
  * done. */
-int64_t knn_q4_search_workspace(int64_t count);
+int64_t knn_q4_search_workspace(int64_t count, int64_t n_queries);
 int knn_q4_search(const knn_q4_rows* q4, int64_t seq, int64_t count, const void* queries,
                   int dtype, int64_t n_queries, int64_t ld, int64_t k, int metric,
                   int64_t* neighbors, float* distances, void* workspace, void* cuda_stream);

@@ -32,8 +32,11 @@ def make_rows(engine, pages=None, **change):
 def test_sizes(engine):
     lib = engine.lib()
     assert [lib.knn_q4_row_bytes(d) for d in (0, 1, 32, 33, 1000, 1024)] == [0, 16, 16, 32, 512, 512]
-    assert lib.knn_q4_search_workspace(-1) == -1
-    assert lib.knn_q4_search_workspace(1) >= 4
+    assert lib.knn_q4_search_workspace(-1, 1) == -1 and lib.knn_q4_search_workspace(1, -1) == -1
+    assert lib.knn_q4_search_workspace(1, 1) >= 4
+    # a key a row and query, for up to 16 queries at once
+    assert 4e6 < lib.knn_q4_search_workspace(10**6, 1) < 5e6
+    assert lib.knn_q4_search_workspace(10**6, 100) == lib.knn_q4_search_workspace(10**6, 16) < 80e6
     p = make_pages(engine)
     # flags' counts, totals and new table rows: room for 4 bytes of each
     assert lib.knn_pages_compact_workspace(ctypes.byref(p), 3, 1000) >= 4 * 3 * (8 + 2)
