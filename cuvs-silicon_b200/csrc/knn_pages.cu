@@ -37,7 +37,7 @@ constexpr int kMaxList = KNN_PAGES_MAX_LIST;
 constexpr int kMoveThreads = 256;
 constexpr int64_t kMoveChunk = 16384;  // bytes of a page that one CTA moves at a time
 constexpr int kShareChunk = 1024;      // table entries that one CTA shares at a time
-constexpr int kKeepChunk = 128;        // positions of a sequence that one CTA compacts
+constexpr int kKeepChunk = 64;         // positions of a sequence that one CTA compacts
 
 // ------------------------------------------------------------ plan kernels
 struct PlanSmem {
@@ -608,11 +608,11 @@ __device__ __forceinline__ void gather_rows(T* pool, const int64_t* from, const 
       if (o >= total) continue;
       const uint32_t r = exact ? __umulhi(o, over) : o / pieces, c = o - r * pieces;
       at[j] = to[r] * pieces + c;
-      v[j] = pool[from[r] * pieces + c];
+      v[j] = __ldcs(pool + from[r] * pieces + c);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (i + j * kMoveThreads < total) pool[at[j]] = v[j];
+      if (i + j * kMoveThreads < total) __stcs(pool + at[j], v[j]);
   }
 }
 
