@@ -851,17 +851,45 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
 #pragma unroll
       for (int i = 0; i < 4; ++i) rows[i] = sh.rows[warp][iteration & 3][g + 8 * i];
       const bool whole = __all_sync(0xffffffffu, (rows[0] | rows[1] | rows[2] | rows[3]) >= 0);
-      if (whole && o.mode == kStore && o.dtype == KNN_DTYPE_F32) {
+      if (whole) {  // all but the last tile: no tests of single rows
+        float norm[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) norm[i] = o.mode == kKeyL2 ? v.norms[rows[i]] : 0.0f;
 #pragma unroll
         for (int c = 0; c < kOutTiles; ++c)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int b = 8 * c + 2 * t + e;
-            if (b >= batch || (kPacked && t >= 2)) continue;
-            float* y = static_cast<float*>(o.y) + b * o.ld + first + g;
-            const float f = sh.inverse[b];
+            const bool real = b < batch && (!kPacked || t < 2);
+            const float f = real ? sh.inverse[b] : 0.0f;
+            const int64_t at = b * o.ld + first + g;
+            float y[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[8 * i] = total[i >> 1][c][2 * (i & 1) + e] * f;
+            for (int i = 0; i < 4; ++i) {
+              y[i] = total[i >> 1][c][2 * (i & 1) + e] * f;
+              if (o.mode != kStore) y[i] = o.mode == kKeyL2 ? norm[i] - 2.0f * y[i] : -y[i];
+            }
+            if (real) {
+              if (o.dtype == KNN_DTYPE_F32) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) static_cast<float*>(o.y)[at + 8 * i] = y[i];
+              } else if (o.dtype == KNN_DTYPE_F16) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  static_cast<__half*>(o.y)[at + 8 * i] = __float2half_rn(y[i]);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  static_cast<__nv_bfloat16*>(o.y)[at + 8 * i] = __float2bfloat16_rn(y[i]);
+              }
+            }
+            if (o.minima) {
+              uint32_t least = min(min(ordered(y[0]), ordered(y[1])), min(ordered(y[2]), ordered(y[3])));
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1)
+                least = min(least, __shfl_xor_sync(0xffffffffu, least, d));
+              if (g == 0 && real) o.minima[b * o.minima_ld + first / kTileRows4] = least;
+            }
           }
         continue;
       }
