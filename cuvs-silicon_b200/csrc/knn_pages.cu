@@ -16,7 +16,10 @@
 // kernels that move data check that word first.
 //
 // What bounds them: planning is a latency (one CTA: a list of a few
-// sequences, a scan of the counts), moving rows is HBM bandwidth.
+// sequences, a scan of the counts; 3 to 8 us), moving rows is HBM bandwidth.
+// Measured: 256 MB of pages copied in 80 to 84 us (513 MB moved, 6.2 TB/s), 210 MB of
+// kept rows gathered in 76 us (420 MB, 5.5 TB/s); 64 children of sequences of
+// 1250 pages forked in 14 us, their freeing included.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -29,8 +32,8 @@ namespace knn {
 namespace {
 
 // Threads of a plan kernel.  Small calls are a chain of loads and barriers:
-// 256 threads go through it faster than 1024 (fork of one sequence 9.3 -> 6 us
-// for the plan), which long lists and many pages need.
+// 256 threads go through it faster than 1024 (the plan of a fork 9.3 -> 6.7 us),
+// which long lists and many pages need.
 constexpr int kFewThreads = 256, kManyThreads = 1024;
 constexpr int64_t kFewList = 1024, kFewPages = 32768;
 constexpr int kMaxList = KNN_PAGES_MAX_LIST;
