@@ -427,15 +427,22 @@ def _stream(device) -> int:
     return _torch().cuda.current_stream(device).cuda_stream
 
 
+def _float_code(name, dtype) -> int:
+    torch = _torch()
+    if dtype is torch.float32:
+        return DTYPE_F32
+    if dtype is torch.float16:
+        return DTYPE_F16
+    if dtype is torch.bfloat16:
+        return DTYPE_BF16
+    raise ValueError(f"{name} of {dtype}: not float32, float16 or bfloat16")
+
+
 def _rows_of(name, t, device, dim):
     """A matrix of vectors (or one vector) of floats whose values lie side by side."""
-    torch = _torch()
-    _on_device(name, t, device, dense=False)
-    dtype = t.dtype
-    code = (DTYPE_F32 if dtype is torch.float32 else DTYPE_F16 if dtype is torch.float16 else
-            DTYPE_BF16 if dtype is torch.bfloat16 else None)
-    if code is None:
-        raise ValueError(f"{name} of {dtype}: not float32, float16 or bfloat16")
+    if not getattr(t, "is_cuda", False) or t.device != device:
+        _on_device(name, t, device, dense=False)
+    code = _float_code(name, t.dtype)
     shape = t.shape
     flat = len(shape) == 1
     if (not flat and len(shape) != 2) or shape[-1] != dim:
@@ -662,12 +669,15 @@ class Q4Rows:
             raise ValueError(f"{count} of {self.n_rows} rows")
         shape = (n, count) if x.dim() == 2 else (count,)
         if out is None:
-            out = torch.empty(shape, dtype=dtype or torch.float32, device=self.device)
-        elif dtype is not None and out.dtype is not dtype:
-            raise ValueError(f"out is {out.dtype}, not {dtype}")
-        elif tuple(out.shape) != shape:
-            raise ValueError(f"out has shape {tuple(out.shape)}, not {shape}")
-        _, ldo, out_code = _rows_of("out", out, self.device, count)
+            dtype = dtype or torch.float32
+            out_code, ldo = _float_code("dtype", dtype), count
+            out = torch.empty(shape, dtype=dtype, device=self.device)
+        else:
+            if dtype is not None and out.dtype is not dtype:
+                raise ValueError(f"out is {out.dtype}, not {dtype}")
+            if tuple(out.shape) != shape:
+                raise ValueError(f"out has shape {tuple(out.shape)}, not {shape}")
+            _, ldo, out_code = _rows_of("out", out, self.device, count)
         _check(lib().knn_q4_products(self._ref, seq, count, x.data_ptr(), code, n, ldx, out.data_ptr(),
                                      out_code, ldo, _stream(self.device)))
         return out
