@@ -644,6 +644,35 @@ def test_pages_fork_of_an_empty_parent_that_is_a_child(torch, engine):
     assert pages.rows.tolist() == [6, 6, 0, 0] and pages.refs.tolist() == [2, 1, 1, 0, 0, 0, 0, 0]
 
 
+@pytest.mark.parametrize("page_rows,rows", [(1, 3000), (16, 5000), (64, 40000)])
+def test_pages_compact_long_sequences_in_place(torch, engine, page_rows, rows):
+    """Calls too large for one plan to do it all: a source that is a target too, and a
+    source of another, while a fork holds its pages."""
+    need = -(-rows // page_rows)
+    pool = torch.zeros(4 * need, page_rows, 2, dtype=torch.int32, device="cuda")
+    pages = engine.Pages.empty([pool], 4, need + 3)
+    pages.grow(ints(torch, (0,)), ints(torch, (rows,)))
+    value = torch.arange(rows, dtype=torch.int32, device="cuda")
+
+    def content(s, n):
+        at = torch.arange(n, device="cuda")
+        return pool[pages.table[s, at // page_rows].long(), at % page_rows]
+
+    at = torch.arange(rows, device="cuda")
+    pool[pages.table[0, at // page_rows].long(), at % page_rows] = torch.stack((value, -value), 1)
+    pages.fork(ints(torch, (0,)), ints(torch, (1,)))
+    keep = randn(torch, 5, 2, rows + 7) > 0.5
+    pages.compact(ints(torch, (0, 0)), ints(torch, (0, 2)), keep)
+    pages.check()
+    for s, want in ((0, value[keep[0, :rows]]), (1, value), (2, value[keep[1, :rows]])):
+        assert int(pages.rows[s]) == len(want)
+        assert torch.equal(content(s, len(want)), torch.stack((want, -want), 1)), s
+    held = pages.table[pages.table >= 0]
+    assert torch.equal(pages.refs, torch.bincount(held, minlength=4 * need).int())
+    pages.free(ints(torch, (0, 1, 2)))
+    assert int(pages.refs.abs().sum()) == 0
+
+
 def test_pages_of_a_large_store(torch, engine):
     """Many pages, lists as long as allowed, a scan over hundreds of thousands of counts."""
     total, n = 300001, 4096
