@@ -401,7 +401,7 @@ __device__ __forceinline__ float put(const Q4Out& o, int64_t b, int64_t i, float
 // Measured (B200; rows of 1024 values in groups of 64, a million of them):
 // 1 to 8 fp16 vectors 117 us, 16 of them 156 us (0.61 of the copy bandwidth
 // that the 608 MB would allow), 16 fp32 ones 244 us; 1 fp32 vector x 10,000
-// rows 7 us.  Copying alone, without the products, takes 92 us.  What bounds it
+// rows 9 us, the call included.  Copying alone, without the products, takes 92 us.  What bounds it
 // is issuing: 350 instructions for 32 rows x 128 codes, of which unpacking is
 // 144, the matrix unit 32 (busy 40% of the time), scaling 32; 12 warps take as
 // long as 16.  Unpacking by ANDs alone, with the zero points taken off by one
@@ -983,7 +983,7 @@ constexpr int kQueryHeld = 8192;  // values up to which a query is kept in share
 
 struct SelectSmem {
   // values 8 i + 2 f and 8 i + 2 f + 1 in [f][i]: lanes take values 8 apart, and
-  // 64 bytes apart they would meet in the banks (rescoring 39k cycles, not 9k)
+  // 64 bytes apart they would meet in the banks (42 us a search's end, not 35)
   double2 query[4][kQueryHeld / 8];  // zeros behind the last value
   uint64_t cand[kCandCap];
   uint32_t pick[kMaxCandidates];  // rows to score again
@@ -1006,7 +1006,8 @@ __device__ __forceinline__ void count_bin(SelectSmem& sm, uint32_t bin) {
 }
 
 // The bin that the value of rank `rank` falls in, (in sm.rank) its rank there
-// and (in sm.inside) how many there are.  All threads; the bins are cleared for the next count.
+// and (in sm.inside) how many there are.  All threads; the bins are cleared for
+// the next count.
 __device__ uint32_t find_bin(SelectSmem& sm, int64_t rank) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int kPer = kBins / kSelectThreads;
@@ -1140,8 +1141,8 @@ __device__ void sort_candidates(SelectSmem& sm, int n) {
   __syncthreads();
 }
 
-// One CTA a query: the k + 16 rows of smallest (key, index), their distances
-// again in 64 bits, and the k first of those.
+// One CTA a query: the k + 16 rows of smallest (key, index), or a few more, their
+// distances again in 64 bits, and the k first of those.
 //
 // The keys' sums are fp32 and rounded; near neighbours lie close together, so
 // that order alone would depend on the order of the sums.  The distances of
