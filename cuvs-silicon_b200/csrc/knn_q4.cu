@@ -1072,7 +1072,10 @@ __device__ uint64_t nth(int64_t n, int64_t rank, SelectSmem& sm, Load load) {
 // more: the range of the minima is cut into 2048 equal bins of their ordered
 // form, the bin of the wanted rank again, until few enough lie at or below its
 // end.  Equal bins of the range that there is, not of a number's bits: minima
-// share those, and atomics on one bin run one after another.
+// share those, and atomics on one bin run one after another.  Where fewer groups
+// than wanted have a key at all (a sequence much shorter than the count, pages
+// missing), the bound is above every key: nothing says how many rows lie at or
+// below the largest minimum.
 __device__ uint32_t minima_bound(const uint32_t* minima, int64_t groups, int wanted,
                                  SelectSmem& sm) {
   auto each = [&](auto&& f) {
@@ -1111,7 +1114,7 @@ __device__ uint32_t minima_bound(const uint32_t* minima, int64_t groups, int wan
     });
     if (threadIdx.x == 0) sm.rank = -1;
     const uint32_t bin = find_bin(sm, rank);
-    if (sm.rank < 0) return high;  // fewer keys than wanted
+    if (sm.rank < 0) return kNoKey - 1;  // fewer keys than wanted
     const uint32_t first = low + (bin << shift);
     const uint32_t last = min(high, first + ((1u << shift) - 1u));
     const int64_t inside = sm.inside;

@@ -1,0 +1,101 @@
+"""Searches of rows in 4 bits where the candidates are hard to tell: a count far
+above the sequence's length.
+
+Expected neighbours come from sums in 64 bits.  Distances are rounded once to
+32 bits: 2^-24 relative.
+"""
+import math
+
+import pytest
+
+from test_gpu_row_store import plain_search, randn, random_rows
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+
+    return torch
+
+
+def check_search(torch, got, values, index, q, k, metric):
+    """The k nearest of `values`, whose positions are `index`; the rest is padding."""
+    near, far = got
+    want, distance, _ = plain_search(torch, values, q, k, metric)
+    want = torch.where(want >= 0, index[want.clamp(min=0)] if len(index) else want, want)
+    assert torch.equal(near, want)
+    fine = want >= 0
+    off = (far.double() - distance).abs()[fine]
+    assert (off <= 2.0 ** -24 * 1.01 * distance.abs()[fine] + 2.0 ** -40).all()
+    assert (far[~fine] == (math.inf if metric == 0 else -math.inf)).all()
+
+
+# ------------------------------------------------- a count above the length
+def long_store(torch, engine, n, room, page_rows, zeros, scale="float16"):
+    """A sequence of n rows of 64 values in a store of `room` rows."""
+    rows, values = random_rows(torch, engine, 100 + n, n, 64, 32, zeros, getattr(torch, scale), page_rows)
+    total = -(-room // page_rows) + 5
+    held, old = [], rows.pages
+    for t in old.pools:
+        p = torch.zeros(total, *t.shape[1:], dtype=t.dtype, device="cuda")
+        p[:t.shape[0]] = t
+        held.append(p)
+    pages = engine.Pages.empty(held, 2, total)
+    pages.table[1, :old.table.shape[1]] = old.table[1]
+    pages.refs[:len(old.refs)] = old.refs
+    pages.rows[1] = n
+    held.insert(2, None) if not zeros else None
+    return engine.Q4Rows(held[0], held[1], 64, 32, held[2], held[3], pages), values
+
+
+@pytest.mark.parametrize("n", [1, 20, 128, 800])
+@pytest.mark.parametrize("metric", [0, 1])
+@pytest.mark.parametrize("page_rows", [48, 256])
+def test_count_far_above_the_length(torch, engine, n, metric, page_rows):
+    rows, values = long_store(torch, engine, n, 100000, page_rows, metric == 1)
+    q = randn(torch, 6, 3, 64)
+    index = torch.arange(n, device="cuda")
+    for count in (900, 3200, 100000):
+        for k in (1, 10, 256):
+            check_search(torch, rows.search(q, k, metric=metric, seq=1, count=count), values[:count],
+                         index[:count], q, k, metric)
+
+
+@pytest.mark.parametrize("metric", [0, 1])
+def test_few_groups_with_keys(torch, engine, metric):
+    """Most rows' pages are missing, or most rows' scales are NaN."""
+    n, page_rows = 20000, 64
+    rows, values = random_rows(torch, engine, 31, n, 64, 32, True, torch.float16, page_rows)
+    q = randn(torch, 6, 5, 64)
+    gone = torch.ones(n // page_rows + 1, dtype=torch.bool, device="cuda")
+    gone[[3, 100, 311]] = False
+    rows.pages.table[1, :len(gone)][gone] = -1
+    index = torch.arange(n, device="cuda")
+    index = index[~gone[index // page_rows]]
+    for k in (1, 10, 100, 256):
+        check_search(torch, rows.search(q, k, metric=metric, seq=1, count=n), values[index], index, q, k, metric)
+    rows, values = random_rows(torch, engine, 32, n, 64, 32, False, torch.float16)
+    keep = torch.zeros(n, dtype=torch.bool, device="cuda")
+    keep[torch.cat((torch.arange(17, 90), torch.tensor([5000]), torch.arange(19001, 19040)))] = True
+    rows.scales[~keep] = float("nan")
+    rows.norms[~keep] = float("nan")
+    index = keep.nonzero().flatten()
+    for k in (1, 10, 100, 256):
+        check_search(torch, rows.search(q, k, metric=metric), values[index], index, q, k, metric)
+
+
+def test_count_above_the_length_in_a_graph(torch, engine):
+    """A captured search of a sequence whose length changes between replays."""
+    rows, values = long_store(torch, engine, 800, 50000, 64, False)
+    q = randn(torch, 6, 4, 64)
+    rows.search(q, 20, seq=1, count=50000)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = rows.search(q, 20, seq=1, count=50000)
+    for n in (800, 37, 0, 260):
+        rows.pages.rows[1] = n
+        graph.replay()
+        check_search(torch, got, values[:n], torch.arange(n, device="cuda"), q, 20, 0)
