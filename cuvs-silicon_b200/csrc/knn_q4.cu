@@ -342,10 +342,10 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Q4View v, Q4List l, floa
 // the order does not depend on |q|^2).
 enum { kStore = 0, kKeyL2 = 1, kKeyProduct = 2 };
 
-// Keys in an order that unsigned numbers have; a key that is +inf or NaN
+// Keys in an order that unsigned numbers have; a key that is no finite number
 // belongs to no neighbour.
 __device__ __forceinline__ uint32_t ordered(float key) {
-  if (!(key < __int_as_float(0x7f800000))) return kNoKey;
+  if (!(fabsf(key) < __int_as_float(0x7f800000))) return kNoKey;
   const uint32_t b = __float_as_uint(key);
   return (b >> 31) ? ~b : b | 0x80000000u;
 }
@@ -1149,7 +1149,10 @@ __device__ void sort_candidates(SelectSmem& sm, int n) {
 //
 // The keys' sums are fp32 and rounded; near neighbours lie close together, so
 // that order alone would depend on the order of the sums.  The distances of
-// the candidates are summed again in 64 bits, which settles it.
+// the candidates are summed again in 64 bits, which settles it.  A candidate
+// whose distance is no finite number in fp32 is dropped then (its key may be:
+// |q|^2 is not in it); a query that is not finite is at no finite distance
+// from any row.
 //
 // Candidates: with c wanted and tau the c-th smallest of the groups' minima,
 // c rows lie at or below tau, so only keys <= tau are looked at, and they are
@@ -1173,12 +1176,16 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
   const int wanted = k + kMoreCandidates;
   uint32_t tau = kNoKey - 1;
   for (int i = threadIdx.x; i < kBins; i += kSelectThreads) sm.hist[i] = 0;
-  for (int j = threadIdx.x; !kWide && j < ((v.dim + 255) & ~255ll); j += kSelectThreads) {
-    const double value = j < v.dim ? static_cast<double>(load_value(x + b * ldx + j)) : 0.0;
-    double2& pair = sm.query[(j & 7) >> 1][j >> 3];
-    (j & 1 ? pair.y : pair.x) = value;
+  bool odd = false;
+  for (int j = threadIdx.x; j < ((v.dim + 255) & ~255ll); j += kSelectThreads) {
+    const float value = j < v.dim ? load_value(x + b * ldx + j) : 0.0f;
+    odd |= !(fabsf(value) < __int_as_float(0x7f800000));
+    if constexpr (!kWide) {
+      double2& pair = sm.query[(j & 7) >> 1][j >> 3];
+      (j & 1 ? pair.y : pair.x) = static_cast<double>(value);
+    }
   }
-  __syncthreads();
+  if (__syncthreads_or(odd)) n = groups = 0;
   if (groups > wanted) tau = min(minima_bound(minima, groups, wanted, sm), kNoKey - 1);
   __syncthreads();
   if (threadIdx.x == 0) sm.count = sm.groups = 0;
@@ -1330,14 +1337,17 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
     if (lane == 0) {
-      if (all != all) all = __longlong_as_double(0x7ff0000000000000ll);
       const uint64_t u = static_cast<uint64_t>(__double_as_longlong(all + 0.0));
-      sm.final_key[warp + kSelectWarps * c] = (u >> 63) ? ~u : u | 0x8000000000000000ull;
+      const bool finite = fabsf(static_cast<float>(all)) < __int_as_float(0x7f800000);
+      sm.final_key[warp + kSelectWarps * c] = !finite ? ~0ull : (u >> 63) ? ~u : u | 0x8000000000000000ull;
       sm.final_row[warp + kSelectWarps * c] = i;
     }
   }
   __syncthreads();
   // the place of each among all, 8 lanes to a candidate
+  int kept = 0;
+  for (int base = 0; base < have; base += kSelectThreads)
+    kept += __syncthreads_count(base + threadIdx.x < have && sm.final_key[base + threadIdx.x] != ~0ull);
   for (int base = 0; base < have; base += kSelectThreads / 8) {
     const int e = base + (threadIdx.x >> 3);
     const uint64_t key = e < have ? sm.final_key[e] : 0;
@@ -1348,14 +1358,14 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
       rank += sm.final_key[o] < key || (sm.final_key[o] == key && sm.final_row[o] < index);
 #pragma unroll
     for (int d = 4; d >= 1; d >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, d);
-    if ((threadIdx.x & 7) == 0 && e < have && rank < k) {
+    if ((threadIdx.x & 7) == 0 && e < have && rank < min(k, kept)) {
       const uint64_t u = (key >> 63) ? key & 0x7fffffffffffffffull : ~key;
       const double d = __longlong_as_double(static_cast<long long>(u));
       neighbors[b * k + rank] = index;
       distances[b * k + rank] = static_cast<float>(kMode == kKeyL2 ? d : -d);
     }
   }
-  for (int e = have + threadIdx.x; e < k; e += kSelectThreads) {
+  for (int e = kept + threadIdx.x; e < k; e += kSelectThreads) {
     neighbors[b * k + e] = -1;
     distances[b * k + e] = __int_as_float(kMode == kKeyL2 ? 0x7f800000 : 0xff800000);
   }

@@ -506,8 +506,9 @@ int knn_q4_products(const knn_q4_rows* q4, int64_t seq, int64_t count, const voi
  * fp32 sums are found first and then ordered by distances summed in 64 bits,
  * which are returned rounded to fp32: the result is the exact one unless 16
  * rows or more lie within fp32's rounding (for L2, of |row|^2 - 2 q.row) at
- * the k-th place.  A row whose distance is no finite number is no
- * neighbour.  L2 needs the norms.  workspace: knn_q4_search_workspace bytes
+ * the k-th place.  A row whose distance (as fp32, or for an
+ * inner product its fp32 sums, and for L2 |row|^2 too) is no finite number is
+ * no neighbour.  L2 needs the norms.  workspace: knn_q4_search_workspace bytes
  * of device memory (16-byte aligned), which this call alone uses until it is
  * done. */
 int64_t knn_q4_search_workspace(int64_t count, int64_t n_queries);

@@ -1,5 +1,5 @@
 """Searches of rows in 4 bits where the candidates are hard to tell: a count far
-above the sequence's length.
+above the sequence's length, and rows without a finite distance.
 
 Expected neighbours come from sums in 64 bits.  Distances are rounded once to
 32 bits: 2^-24 relative.
@@ -99,3 +99,73 @@ def test_count_above_the_length_in_a_graph(torch, engine):
         rows.pages.rows[1] = n
         graph.replay()
         check_search(torch, got, values[:n], torch.arange(n, device="cuda"), q, 20, 0)
+
+
+# ------------------------------------------- distances that are no finite number
+@pytest.mark.parametrize("metric", [0, 1])
+@pytest.mark.parametrize("x", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("dim", [64, 9001])
+def test_queries_that_are_not_finite(torch, engine, metric, x, dim):
+    """No row is at a finite distance from them; the queries beside them find theirs."""
+    rows, values = random_rows(torch, engine, 41, 3000, dim, 32, True, torch.float16)
+    q = randn(torch, 6, 5, dim).to(getattr(torch, x))
+    q[1, 7], q[2, dim - 1], q[3, 0] = math.inf, -math.inf, math.nan
+    near, far = rows.search(q, 30, metric=metric)
+    index = torch.arange(3000, device="cuda")
+    check_search(torch, (near[::4], far[::4]), values, index, q[::4], 30, metric)
+    assert (near[1:4] == -1).all()
+    assert (far[1:4] == (math.inf if metric == 0 else -math.inf)).all()
+
+
+@pytest.mark.parametrize("metric", [0, 1])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_rows_that_are_not_finite(torch, engine, metric, zeros):
+    """Scales of both infinities among the rows, more of them than are looked for."""
+    n = 5000
+    rows, values = random_rows(torch, engine, 42, n, 96, 32, zeros, torch.float16)
+    odd = torch.arange(n, device="cuda") % 3 != 1
+    rows.scales[odd, 1] = math.inf
+    rows.scales[::6, 1] = -math.inf
+    rows.norms[odd] = math.inf
+    index = (~odd).nonzero().flatten()
+    q = randn(torch, 6, 4, 96)
+    for k in (1, 40, 256):
+        check_search(torch, rows.search(q, k, metric=metric), values[index], index, q, k, metric)
+
+
+def test_distances_beyond_32_bits(torch, engine):
+    """Products and squares that 64 bits hold and 32 do not: such rows are no
+    neighbours either, and the others keep their order."""
+    n = 4000
+    rows, _ = random_rows(torch, engine, 43, n, 64, 32, False, torch.float16)
+    rows.scales[:] = torch.where(torch.arange(n, device="cuda")[:, None] % 4 == 0, 0.5, 2.0).half()
+    values = rows.read().double()
+    rows.norms[:] = values.square().sum(1).float()
+    q = torch.zeros(2, 64, device="cuda")
+    q[0, 5], q[1, 40] = 1.5e38, -2.5e38
+    q[:, 9] = 1e36
+    most = torch.finfo(torch.float32).max
+    for b in (0, 1):
+        product = values @ q[b].double()
+        index = (product.abs() <= most).nonzero().flatten()
+        assert 500 < len(index) < 3500
+        for k in (10, 256):
+            check_search(torch, rows.search(q[b:b + 1], k, metric=1), values[index], index, q[b:b + 1], k, 1)
+    # squares: every distance is too large, though |row|^2 - 2 q.row is not
+    near, far = rows.search(torch.full((1, 64), 3e18, device="cuda"), 10)
+    assert (near == -1).all() and torch.isinf(far).all()
+    # some are not: |q|^2 = 2^128, and a value above 0 takes 2^105 or more off it
+    rows, _ = random_rows(torch, engine, 44, n, 64, 32, False, torch.bfloat16)
+    rows.scales[:] = 2.0 ** 40
+    values = rows.read().double()
+    rows.norms[:] = values.square().sum(1).float()
+    q = torch.zeros(1, 64, device="cuda")
+    q[0, 3] = 2.0 ** 64
+    near, far = rows.search(q, 100)
+    assert torch.isfinite(far).all() and (values[near[0], 3] > 0).all()
+    keep = values[:, 3] > 0
+    keep[keep.nonzero().flatten()[50:]] = False
+    rows.scales[~keep & (values[:, 3] > 0)] = math.nan  # 50 rows are left at finite distances
+    near, far = rows.search(q, 100)
+    assert torch.equal(near[0, :50].sort().values, keep.nonzero().flatten())
+    assert torch.isfinite(far[0, :50]).all() and (near[0, 50:] == -1).all() and torch.isinf(far[0, 50:]).all()
