@@ -383,7 +383,10 @@ __device__ __forceinline__ float put(const Q4Out& o, int64_t b, int64_t i, float
 // two of its own that brings its largest finite magnitude to 2^14 .. 2^15,
 // and fp32 ones split into two fp16 parts (columns of their own, added up
 // after the group's scaling): x = high + low is off by at most 2^-24 |x| +
-// 2^-40 max|x|, a bf16 one by 2^-40 max|x| at the very most.
+// 2^-40 max|x|, a bf16 one by 2^-40 max|x| at the very most.  Small vectors
+// are scaled up, and a bf16 scale can be so large that only the product comes
+// down again: such a group's sum is first scaled back by up to 2^-40, which is
+// exact and keeps 2^19 values of any size in range.
 //
 // A warp takes tiles of 32 rows and runs down their codes in stages of 256,
 // which it copies ahead into a ring of its own in shared memory (cp.async, no
@@ -428,7 +431,9 @@ struct MmaPlan {
 // [kSumStride], then the vectors.
 struct MmaShared {
   uint32_t largest[kQ4SearchBatch];
-  float factor[kQ4SearchBatch], inverse[kQ4SearchBatch];
+  // a vector's power of two, and its inverse in two steps: taken off a group's
+  // sum before the scale multiplies it (bf16 scales), and off the product
+  float factor[kQ4SearchBatch], early[kQ4SearchBatch], inverse[kQ4SearchBatch];
   // rows of the tiles that a warp is at, by iteration: it copies ahead by up
   // to two stages, so by as many tiles
   int32_t rows[kMmaWarps][4][kTileRows4];
@@ -645,7 +650,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   };
   // ---- the vectors' scales
   if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
-    if (threadIdx.x < kQ4SearchBatch) sh.factor[threadIdx.x] = sh.inverse[threadIdx.x] = 1.0f;
+    if (threadIdx.x < kQ4SearchBatch)
+      sh.factor[threadIdx.x] = sh.early[threadIdx.x] = sh.inverse[threadIdx.x] = 1.0f;
     __syncthreads();
   } else {
     __syncthreads();
@@ -663,8 +669,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       const uint32_t most = sh.largest[threadIdx.x];
       int e = most ? 14 - (static_cast<int>(most >> 23) - 127) : 0;
       if (e > 126) e = 126;
+      const int first = v.scale_bf16 && e > 0 ? (e < 40 ? e : 40) : 0;
       sh.factor[threadIdx.x] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-      sh.inverse[threadIdx.x] = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      sh.early[threadIdx.x] = __uint_as_float(static_cast<uint32_t>(127 - first) << 23);
+      sh.inverse[threadIdx.x] = __uint_as_float(static_cast<uint32_t>(127 - e + first) << 23);
     }
     __syncthreads();
   }
@@ -842,6 +850,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
                 for (int e = 0; e < 2; ++e) {
                   float sum = acc[m][c][h + e];
                   if constexpr (!kPacked && kParts == 2) sum += acc[m][c + kOutTiles][h + e];
+                  if constexpr (!std::is_same<T, __half>::value)
+                    if (v.scale_bf16) sum *= sh.early[kPacked ? (2 * t + e) & 3 : 8 * c + 2 * t + e];
                   total[m][c][h + e] = fmaf(scale[i], sum, total[m][c][h + e]);
                 }
             }
