@@ -382,8 +382,13 @@ __device__ __forceinline__ float put(const Q4Out& o, int64_t b, int64_t i, float
 // they are; bf16 and fp32 ones are first scaled, each vector by a power of
 // two of its own that brings its largest finite magnitude to 2^14 .. 2^15,
 // and fp32 ones split into two fp16 parts (columns of their own, added up
-// after the group's scaling): x = high + low is off by at most 2^-24 |x| +
-// 2^-40 max|x|, a bf16 one by 2^-40 max|x| at the very most.  Small vectors
+// at the group's end): high, and what is left, at most 8, times 2^12, so that it
+// has 11 bits too where the value is small.  Two parts of 11 bits and a sign
+// hold a value to 2^-23 of it; fp16's smallest step, 2^-24, is 2^-50 of the
+// largest value in the low part, so x is off by at most 2^-23 |x| + 2^-51
+// max|x|: a value has fewer bits only where it is 2^28 below its vector's
+// largest, which the sums of a row that is zero at the large ones can show.  A
+// bf16 value has 8 bits, and is exact but for 2^-39 max|x|.  Small vectors
 // are scaled up, and a bf16 scale can be so large that only the product comes
 // down again: such a group's sum is first scaled back by up to 2^-40, which is
 // exact and keeps 2^19 values of any size in range.
@@ -415,6 +420,7 @@ constexpr int kTileRows4 = 32;    // rows of a tile
 constexpr int kStageCodes = 256;  // codes of a row in a stage: two halves
 constexpr int kStageBytes4 = kTileRows4 * kStageCodes / 2;
 constexpr int kRing = 2;          // the stage at hand and the next
+constexpr float kLowUp = 4096.0f;  // what an fp32 vector's low part is multiplied by
 constexpr int kSumStride = 36;    // floats from column to column of a tile's sums: no bank twice
 
 struct MmaPlan {
@@ -722,7 +728,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         h[e] = __float2half_rn(scaled);
         if (kParts == 2 && low) {
           const float high = __half2float(h[e]);
-          h[e] = __float2half_rn(fabsf(high) <= 65504.0f ? scaled - high : 0.0f);
+          h[e] = __float2half_rn(fabsf(high) <= 65504.0f ? (scaled - high) * kLowUp : 0.0f);
         }
       }
       uint4 out;
@@ -849,7 +855,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                   float sum = acc[m][c][h + e];
-                  if constexpr (!kPacked && kParts == 2) sum += acc[m][c + kOutTiles][h + e];
+                  if constexpr (!kPacked && kParts == 2)
+                    sum = fmaf(acc[m][c + kOutTiles][h + e], 1.0f / kLowUp, sum);
                   if constexpr (!std::is_same<T, __half>::value)
                     if (v.scale_bf16) sum *= sh.early[kPacked ? (2 * t + e) & 3 : 8 * c + 2 * t + e];
                   total[m][c][h + e] = fmaf(scale[i], sum, total[m][c][h + e]);
@@ -864,7 +871,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          total[m][0][e] += __shfl_xor_sync(0xffffffffu, total[m][0][e], 2);
+          total[m][0][e] =
+              fmaf(__shfl_xor_sync(0xffffffffu, total[m][0][e], 2), 1.0f / kLowUp, total[m][0][e]);
     }
     const int64_t first = tile_of(iteration) * kTileRows4;
     if (p.split == 1) {

@@ -493,7 +493,8 @@ int knn_q4_read(const knn_q4_rows* q4, const int32_t* seqs, const int32_t* count
 
 /* Products of `batch` vectors (vector b at x + b * ldx) with rows 0 .. count
  * - 1: out[b * ldo + i] = row i . x_b, summed in fp32 and rounded once to
- * out_dtype.  In pages: rows of sequence `seq`; beyond its length 0 is
+ * out_dtype.  fp16 vectors are taken as they are; an fp32 one is held to
+ * 2^-23 |x_j| + 2^-51 max|x| in each value, a bf16 one to 2^-39 max|x|.  In pages: rows of sequence `seq`; beyond its length 0 is
  * written, and a row whose page is missing gives NaN.  Dense rows: seq = -1. */
 int knn_q4_products(const knn_q4_rows* q4, int64_t seq, int64_t count, const void* x, int dtype,
                     int64_t batch, int64_t ldx, void* out, int out_dtype, int64_t ldo,
