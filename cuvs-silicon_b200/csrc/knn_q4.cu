@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Q4View v, Q4List l, floa
 // --------------------------------------------------------------- products
 // What becomes of a product: stored (in the output's type), or the key that a
 // search orders rows by, |row|^2 - 2 q.row or -q.row (fp32; a row's place in
-// the order does not depend on |q|^2).
+// the order does not depend on |q|^2), less a bound of its error.
 enum { kStore = 0, kKeyL2 = 1, kKeyProduct = 2 };
 
 // Keys in an order that unsigned numbers have; a key that is no finite number
@@ -355,19 +355,44 @@ struct Q4Out {
   int dtype;
   int64_t ld;
   int mode;
-  uint32_t* minima;  // [vectors][minima_ld]: smallest key of each tile of 32 rows, or nullptr
+  uint32_t* minima;  // [vectors][minima_ld]: smallest key of each tile of 32 rows
   int64_t minima_ld;
+  // keys: a key's error over |x| |row| (products: over sum |x_j| and the row's
+  // largest scale), and over |row|^2
+  float slack, norm_slack;
 };
 
-// Stores a product, or makes it a key, which it stores and returns.
-__device__ __forceinline__ float put(const Q4Out& o, int64_t b, int64_t i, float y, float norm) {
-  if (o.mode == kKeyL2) y = norm - 2.0f * y;
-  if (o.mode == kKeyProduct) y = -y;
+__device__ __forceinline__ float root(float a) {
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(a));
+  return r;
+}
+
+// A lower bound of the true key.  It is the key less what the sums can be off
+// by: with steps = 2 group + groups + 32, at most
+//   steps 2^-23 sum_j |x_j row_j|
+// (a group's values pass through group / 16 matrix instructions that cut 17
+// numbers each at 2^-23 of their magnitudes or better, the groups' sums
+// through one rounding for each group that follows; the vector's own rounding,
+// the splits' adding up and the key's arithmetic are in the 32), and for L2
+// what |row|^2 is off by as it is held.  The sum is at most |x| |row|, and for
+// products, which need no norms, at most sum |x_j| times 15 (8 without zero
+// points) times the row's largest scale.  `size` is |row| or that scale,
+// `reach` what it is multiplied by.
+__device__ __forceinline__ float lowest_key(const Q4Out& o, float y, float norm, float reach, float size) {
+  constexpr float kMost = 3.402823466e38f, kTiny = 0x1p-140f;  // kTiny: subnormal sums
+  const float key = o.mode == kKeyL2 ? norm - 2.0f * y : -y;
+  const float extra = o.mode == kKeyL2 ? fmaf(o.norm_slack, norm, kTiny) : kTiny;
+  const float low = fmaxf(key - fminf(fmaf(reach, size, extra), kMost), -kMost);
+  return fabsf(key) <= kMost ? low : __int_as_float(0x7fc00000);
+}
+
+// Stores a product or a key.
+__device__ __forceinline__ void put(const Q4Out& o, int64_t b, int64_t i, float y) {
   const int64_t at = b * o.ld + i;
   if (o.dtype == KNN_DTYPE_F32) static_cast<float*>(o.y)[at] = y;
   else if (o.dtype == KNN_DTYPE_F16) static_cast<__half*>(o.y)[at] = __float2half_rn(y);
   else static_cast<__nv_bfloat16*>(o.y)[at] = __float2bfloat16_rn(y);
-  return y;
 }
 
 // The products run on the warp's own matrix instructions (mma.sync, fp16 in,
@@ -419,6 +444,7 @@ constexpr int kMmaThreads = 32 * kMmaWarps;
 constexpr int kTileRows4 = 32;    // rows of a tile
 constexpr int kStageCodes = 256;  // codes of a row in a stage: two halves
 constexpr int kStageBytes4 = kTileRows4 * kStageCodes / 2;
+static_assert(kMmaWarps == kQ4SearchBatch, "a warp to a vector");
 constexpr int kRing = 2;          // the stage at hand and the next
 constexpr float kLowUp = 4096.0f;  // what an fp32 vector's low part is multiplied by
 constexpr int kSumStride = 36;    // floats from column to column of a tile's sums: no bank twice
@@ -434,12 +460,14 @@ struct MmaPlan {
 
 // Dynamic shared memory: ring[warp][kRing][kStageBytes4], then scales[warp][2]
 // [groups of a stage][32 rows], then (split > 1) sums[warp][vector]
-// [kSumStride], then the vectors.
+// [kSumStride] and for keys of products largest[warp][kSumStride], then the
+// vectors.  Before the ring is used, mosts[vector][warp] and sizes[vector][warp]
+// lie in its place.
 struct MmaShared {
-  uint32_t largest[kQ4SearchBatch];
   // a vector's power of two, and its inverse in two steps: taken off a group's
   // sum before the scale multiplies it (bf16 scales), and off the product
   float factor[kQ4SearchBatch], early[kQ4SearchBatch], inverse[kQ4SearchBatch];
+  float reach[kQ4SearchBatch];  // of a vector's keys
   // rows of the tiles that a warp is at, by iteration: it copies ahead by up
   // to two stages, so by as many tiles
   int32_t rows[kMmaWarps][4][kTileRows4];
@@ -514,7 +542,8 @@ struct HeldScales {
 // kParts: fp16 parts of a vector.  With kTiles = 1 and two parts, columns 0-3
 // hold the high parts of 4 vectors and 4-7 the low ones; otherwise the tiles'
 // first half holds the high parts.  kGroups: groups in half a stage (128 / group).
-template <class T, int kTiles, int kParts, int kGroups, bool kZeros>
+// kKeyed: keys (o.mode says which), not products to store.
+template <class T, int kTiles, int kParts, int kGroups, bool kZeros, bool kKeyed>
 __global__ void __launch_bounds__(kMmaThreads, 1)
     products_kernel(Q4View v, Q4Range r, const T* x, int batch, int64_t ldx, Q4Out o, MmaPlan p) {
   constexpr bool kPacked = kTiles == 1 && kParts == 2;
@@ -530,10 +559,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
                      warp * (2 * kScales);
   float* sums = reinterpret_cast<float*>(raw + kMmaWarps * (kRing * kStageBytes4 + 2 * kScales * 4));
   const int sum_words = batch * kSumStride;  // of a warp
-  uint4* vectors = reinterpret_cast<uint4*>(sums + (p.split > 1 ? kMmaWarps * sum_words : 0));
+  float* largest = sums + kMmaWarps * sum_words;
+  uint4* vectors = reinterpret_cast<uint4*>(
+      p.split == 1 ? sums : largest + (kKeyed && o.mode == kKeyProduct ? kMmaWarps * kSumStride : 0));
   const int slots = kMmaWarps / p.split, slot = warp / p.split, part = warp % p.split;
 
-  if (threadIdx.x < kQ4SearchBatch) sh.largest[threadIdx.x] = 0;
   wait_for_stream();
   int64_t n = r.count;
   if (r.length) n = *r.length < n ? *r.length : n;
@@ -654,34 +684,63 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       }
     }
   };
-  // ---- the vectors' scales
-  if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
-    if (threadIdx.x < kQ4SearchBatch)
-      sh.factor[threadIdx.x] = sh.early[threadIdx.x] = sh.inverse[threadIdx.x] = 1.0f;
-    __syncthreads();
-  } else {
-    __syncthreads();
-    for (int b = 0; b < batch; ++b) {
+  // ---- the vectors' powers of two, and what their keys can be off by: 16 /
+  // batch warps read a vector, and a warp adds up what they found
+  constexpr bool kAsHeld = std::is_same<T, __half>::value;
+  if constexpr (!kAsHeld || kKeyed) {
+    uint32_t* mosts = reinterpret_cast<uint32_t*>(raw);
+    float* sizes = reinterpret_cast<float*>(raw) + kMmaWarps * kQ4SearchBatch;
+    int shift = 4;
+    while ((batch << shift) > kMmaWarps) --shift;
+    const int each = 1 << shift, part = warp & (each - 1), from_vector = warp >> shift;
+    if (from_vector < batch) {
       uint32_t most = 0;
-      for (int64_t j = threadIdx.x; j < v.dim; j += kMmaThreads) {
-        const uint32_t bits = __float_as_uint(load_value(x + b * ldx + j)) & 0x7fffffffu;
-        if (bits < 0x7f800000u && bits > most) most = bits;
+      float size = 0.0f;
+      for (int base = 32 * part + lane; base < static_cast<int>(v.dim); base += 128 << shift) {
+        float a[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int j = base + (u << (shift + 5));
+          a[u] = j < static_cast<int>(v.dim) ? load_value(x + from_vector * ldx + j) : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const uint32_t bits = __float_as_uint(a[u]) & 0x7fffffffu;
+          if (!kAsHeld && bits < 0x7f800000u && bits > most) most = bits;
+          if constexpr (kKeyed) size = o.mode == kKeyL2 ? fmaf(a[u], a[u], size) : size + fabsf(a[u]);
+        }
       }
-      most = __reduce_max_sync(0xffffffffu, most);
-      if (lane == 0 && most) atomicMax(&sh.largest[b], most);
+      if constexpr (!kAsHeld) most = __reduce_max_sync(0xffffffffu, most);
+      if constexpr (kKeyed) {
+#pragma unroll
+        for (int d = 16; d >= 1; d >>= 1) size += __shfl_xor_sync(0xffffffffu, size, d);
+      }
+      if (lane == 0) {
+        mosts[from_vector * kMmaWarps + part] = most;
+        sizes[from_vector * kMmaWarps + part] = size;
+      }
     }
     __syncthreads();
-    if (threadIdx.x < kQ4SearchBatch) {
-      const uint32_t most = sh.largest[threadIdx.x];
+    const bool mine_too = warp < batch && lane < each;
+    const uint32_t most = __reduce_max_sync(0xffffffffu, mine_too ? mosts[warp * kMmaWarps + lane] : 0);
+    float size = mine_too ? sizes[warp * kMmaWarps + lane] : 0.0f;
+#pragma unroll
+    for (int d = 8; d >= 1; d >>= 1) size += __shfl_xor_sync(0xffffffffu, size, d);
+    if (lane == 0) {
       int e = most ? 14 - (static_cast<int>(most >> 23) - 127) : 0;
       if (e > 126) e = 126;
       const int first = v.scale_bf16 && e > 0 ? (e < 40 ? e : 40) : 0;
-      sh.factor[threadIdx.x] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-      sh.early[threadIdx.x] = __uint_as_float(static_cast<uint32_t>(127 - first) << 23);
-      sh.inverse[threadIdx.x] = __uint_as_float(static_cast<uint32_t>(127 - e + first) << 23);
+      sh.factor[warp] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+      sh.early[warp] = __uint_as_float(static_cast<uint32_t>(127 - first) << 23);
+      sh.inverse[warp] = __uint_as_float(static_cast<uint32_t>(127 - e + first) << 23);
+      // squares below 2^-149 are lost: 2^-66 is what 2^16 of them can come to
+      if (kKeyed && o.mode == kKeyL2) size = root(size) + 0x1p-66f;
+      if constexpr (kKeyed) sh.reach[warp] = o.slack * size;
     }
-    __syncthreads();
+  } else if (threadIdx.x < kQ4SearchBatch) {
+    sh.factor[threadIdx.x] = sh.early[threadIdx.x] = sh.inverse[threadIdx.x] = 1.0f;
   }
+  __syncthreads();
 
   // ---- a chunk of the vectors, as the matrix instruction takes them
   const bool wide = ((reinterpret_cast<uintptr_t>(x) | (ldx * sizeof(T))) & 15) == 0;
@@ -750,6 +809,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   uint32_t scales_now = 0;  // words into the scales
   for (int iteration = 0; iteration < p.iterations; ++iteration) {
     float total[2][kOutTiles][4] = {};
+    float most_scale[4] = {};  // of rows g + 8 i, for keys of products
     for (int chunk = 0; chunk < p.chunks; ++chunk) {
       if (p.chunks > 1 && (iteration > 0 || chunk > 0)) {
         __syncthreads();
@@ -819,6 +879,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
                 sixteen[i] = 0xd480d480u;
               }
             }
+            if constexpr (kKeyed) {  // for both keys: a branch costs more
+#pragma unroll
+              for (int i = 0; i < 4; ++i) most_scale[i] = fmaxf(most_scale[i], fabsf(scale[i]));
+            }
 #pragma unroll
             for (int w = j * kPerGroup; w < (j + 1) * kPerGroup; ++w) {
               uint32_t a[4][4];
@@ -882,25 +946,30 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       for (int i = 0; i < 4; ++i) rows[i] = sh.rows[warp][iteration & 3][g + 8 * i];
       const bool whole = __all_sync(0xffffffffu, (rows[0] | rows[1] | rows[2] | rows[3]) >= 0);
       if (whole) {  // all but the last tile: no tests of single rows
-        float norm[4];
+        [[maybe_unused]] float norm[4], size[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) norm[i] = o.mode == kKeyL2 ? v.norms[rows[i]] : 0.0f;
+        for (int i = 0; kKeyed && i < 4; ++i) {
+          norm[i] = o.mode == kKeyL2 ? v.norms[rows[i]] : 0.0f;
+          size[i] = o.mode == kKeyL2 ? root(norm[i]) : most_scale[i];
+        }
 #pragma unroll
         for (int c = 0; c < kOutTiles; ++c)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
+            if (8 * c + e >= batch) continue;  // no lane has a vector
             const int b = 8 * c + 2 * t + e;
             const bool real = b < batch && (!kPacked || t < 2);
             const float f = real ? sh.inverse[b] : 0.0f;
+            [[maybe_unused]] const float reach = kKeyed && real ? sh.reach[b] : 0.0f;
             const int64_t at = b * o.ld + first + g;
             float y[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               y[i] = total[i >> 1][c][2 * (i & 1) + e] * f;
-              if (o.mode != kStore) y[i] = o.mode == kKeyL2 ? norm[i] - 2.0f * y[i] : -y[i];
+              if constexpr (kKeyed) y[i] = lowest_key(o, y[i], norm[i], reach, size[i]);
             }
             if (real) {
-              if (o.dtype == KNN_DTYPE_F32) {
+              if (kKeyed || o.dtype == KNN_DTYPE_F32) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) static_cast<float*>(o.y)[at + 8 * i] = y[i];
               } else if (o.dtype == KNN_DTYPE_F16) {
@@ -913,7 +982,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
                   static_cast<__nv_bfloat16*>(o.y)[at + 8 * i] = __float2bfloat16_rn(y[i]);
               }
             }
-            if (o.minima) {
+            if constexpr (kKeyed) {
               uint32_t least = min(min(ordered(y[0]), ordered(y[1])), min(ordered(y[2]), ordered(y[3])));
 #pragma unroll
               for (int d = 4; d < 32; d <<= 1)
@@ -936,10 +1005,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
             if (!mine_too || at >= r.count) continue;
             float y = total[i >> 1][c][2 * (i & 1) + e] * sh.inverse[b];
             if (rows[i] < 0) y = at < n ? __int_as_float(0x7fc00000) : 0.0f;
-            const float key = put(o, b, at, y, o.mode == kKeyL2 && rows[i] >= 0 ? v.norms[rows[i]] : 0.0f);
-            if (at < n) least = min(least, ordered(key));
+            if constexpr (kKeyed) {
+              const float norm = o.mode == kKeyL2 && rows[i] >= 0 ? v.norms[rows[i]] : 0.0f;
+              y = lowest_key(o, y, norm, sh.reach[b], o.mode == kKeyL2 ? root(norm) : most_scale[i]);
+            }
+            put(o, b, at, y);
+            if (at < n) least = min(least, ordered(y));
           }
-          if (o.minima) {
+          if constexpr (kKeyed) {
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1)
               least = min(least, __shfl_xor_sync(0xffffffffu, least, d));
@@ -958,6 +1031,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
           for (int i = 0; i < 4; ++i)
             own[b * kSumStride + g + 8 * i] = total[i >> 1][c][2 * (i & 1) + e];
         }
+      if (kKeyed && o.mode == kKeyProduct && t == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) largest[warp * kSumStride + g + 8 * i] = most_scale[i];
+      }
       __syncthreads();
       // a warp to a tile and vector, a lane to a row
       for (int item = warp; item < slots * batch; item += kMmaWarps) {
@@ -973,10 +1050,18 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         if (at_row < 0) y = at < n ? __int_as_float(0x7fc00000) : 0.0f;
         uint32_t least = kNoKey;
         if (at < r.count) {
-          const float key = put(o, b, at, y, o.mode == kKeyL2 && at_row >= 0 ? v.norms[at_row] : 0.0f);
-          if (at < n) least = ordered(key);
+          if constexpr (kKeyed) {
+            const float norm = o.mode == kKeyL2 && at_row >= 0 ? v.norms[at_row] : 0.0f;
+            float size = root(norm);
+            if (o.mode == kKeyProduct)
+              for (int q = 0; q < p.split; ++q)
+                size = fmaxf(size, largest[(s * p.split + q) * kSumStride + lane]);
+            y = lowest_key(o, y, norm, sh.reach[b], size);
+          }
+          put(o, b, at, y);
+          if (at < n) least = ordered(y);
         }
-        if (o.minima) {
+        if constexpr (kKeyed) {
           least = __reduce_min_sync(0xffffffffu, least);
           if (lane == 0) o.minima[b * o.minima_ld + tile] = least;
         }
@@ -991,9 +1076,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
 constexpr int kGroupRows = kTileRows4;  // rows whose smallest key is kept
 constexpr int kSelectThreads = 1024;
 constexpr int kMoreCandidates = 16;  // scored again beyond the k asked for
-constexpr int kMaxCandidates = KNN_MAX_K + 2 * kMoreCandidates;
-constexpr int kGroupCap = 1024;
+constexpr int kScoreCap = 1024;      // rows that are scored at a time
+constexpr int kGroupCap = 1024;  // kSelectThreads at least: one group a thread is listed at a time
 constexpr int kCandCap = 4096;
+static_assert(kGroupCap >= kSelectThreads && kScoreCap <= 32 * 32 && kScoreCap >= KNN_MAX_K + 2 * kMoreCandidates);
 constexpr int kRankCap = 512;  // candidates that are ranked by counting, not sorted
 
 constexpr int kBins = 2048;
@@ -1004,14 +1090,19 @@ struct SelectSmem {
   // 64 bytes apart they would meet in the banks (42 us a search's end, not 35)
   double2 query[4][kQueryHeld / 8];  // zeros behind the last value
   uint64_t cand[kCandCap];
-  uint32_t pick[kMaxCandidates];  // rows to score again
-  uint64_t final_key[kMaxCandidates];
-  uint32_t final_row[kMaxCandidates];
+  uint32_t pick[kScoreCap];  // rows to score again
+  // the nearest so far, and those just scored
+  uint64_t final_key[KNN_MAX_K + kScoreCap];
+  uint32_t final_row[KNN_MAX_K + kScoreCap];
+  uint64_t best_key[KNN_MAX_K];
+  uint32_t best_row[KNN_MAX_K];
+  float squared;    // |q|^2 from below
+  uint32_t absent;  // scored rows that are at no finite distance
   uint32_t hist[kBins];
   uint32_t part[32];
   int32_t group[kGroupCap];
   uint32_t count, groups;
-  uint64_t prefix;
+  uint64_t prefix, last;
   int64_t rank;
   int64_t inside;  // values in the bin
 };
@@ -1169,8 +1260,17 @@ __device__ void sort_candidates(SelectSmem& sm, int n) {
 // that order alone would depend on the order of the sums.  The distances of
 // the candidates are summed again in 64 bits, which settles it.  A candidate
 // whose distance is no finite number in fp32 is dropped then (its key may be:
-// |q|^2 is not in it); a query that is not finite is at no finite distance
-// from any row.
+// |q|^2 is not in it).  A query that is not finite makes no key that is.
+//
+// Keys are lower bounds, so a row is no neighbour if its key is above the k-th
+// distance (less |q|^2).  Mostly that holds for every row that is no
+// candidate.  Where it does not (near copies of one row, rows whose sums
+// cancel), the other rows with keys up to that distance are scored too, up to
+// 1024 at a time, while the k-th distance comes down: the result is the exact
+// one always, and such a search takes longer the more rows there are that
+// fp32 cannot tell apart (a million rows of 1024 values, one query, k = 10: 0.15
+// ms, with 1000 copies of the nearest 0.32, with 10,000 of them 3.8, with 100,000
+// 18).
 //
 // Candidates: with c wanted and tau the c-th smallest of the groups' minima,
 // c rows lie at or below tau, so only keys <= tau are looked at, and they are
@@ -1194,16 +1294,14 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
   const int wanted = k + kMoreCandidates;
   uint32_t tau = kNoKey - 1;
   for (int i = threadIdx.x; i < kBins; i += kSelectThreads) sm.hist[i] = 0;
-  bool odd = false;
-  for (int j = threadIdx.x; j < ((v.dim + 255) & ~255ll); j += kSelectThreads) {
-    const float value = j < v.dim ? load_value(x + b * ldx + j) : 0.0f;
-    odd |= !(fabsf(value) < __int_as_float(0x7f800000));
-    if constexpr (!kWide) {
-      double2& pair = sm.query[(j & 7) >> 1][j >> 3];
-      (j & 1 ? pair.y : pair.x) = static_cast<double>(value);
-    }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int j = threadIdx.x; !kWide && j < ((v.dim + 255) & ~255ll); j += kSelectThreads) {
+    const double value = j < v.dim ? static_cast<double>(load_value(x + b * ldx + j)) : 0.0;
+    double2& pair = sm.query[(j & 7) >> 1][j >> 3];
+    (j & 1 ? pair.y : pair.x) = value;
   }
-  if (__syncthreads_or(odd)) n = groups = 0;
+  if (threadIdx.x == 0) sm.absent = 0;
+  __syncthreads();
   if (groups > wanted) tau = min(minima_bound(minima, groups, wanted, sm), kNoKey - 1);
   __syncthreads();
   if (threadIdx.x == 0) sm.count = sm.groups = 0;
@@ -1234,13 +1332,14 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
     __syncthreads();
   }
   constexpr int kSelectWarps = kSelectThreads / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int have;
+  uint64_t last;  // (key, index) of the last candidate, all ones where there are no other rows
   if (listed <= kGroupCap && sm.count <= kCandCap) {
     const int count = static_cast<int>(sm.count);
     have = min(count, wanted);
     if (count <= wanted + kMoreCandidates) {  // a few more do no harm
       have = count;
+      last = tau == kNoKey - 1 ? ~0ull : static_cast<uint64_t>(tau) << 32 | 0xffffffffu;
       for (int e = threadIdx.x; e < count; e += kSelectThreads)
         sm.pick[e] = static_cast<uint32_t>(sm.cand[e]);
     } else if (count <= kRankCap) {
@@ -1251,7 +1350,10 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
         for (int o = lane; o < count; o += 32) before += sm.cand[o] < c;
         before = __reduce_add_sync(0xffffffffu, before);
         if (lane == 0 && before < wanted) sm.pick[before] = static_cast<uint32_t>(c);
+        if (lane == 0 && before == wanted - 1) sm.last = c;
       }
+      __syncthreads();
+      last = sm.last;
     } else {
       int size = 2;
       while (size < count) size <<= 1;
@@ -1259,6 +1361,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
       sort_candidates(sm, size);
       for (int e = threadIdx.x; e < have; e += kSelectThreads)
         sm.pick[e] = static_cast<uint32_t>(sm.cand[e]);
+      last = sm.cand[wanted - 1];
     }
   } else {
     // many equal keys: the row of rank wanted - 1 by (key, index), over all rows
@@ -1266,7 +1369,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
       const uint32_t key = ordered(keys[i]);
       return (static_cast<uint64_t>(key) << 32) | static_cast<uint32_t>(i);
     };
-    const uint64_t last = n > wanted ? nth(n, wanted - 1, sm, load) : ~0ull;
+    last = n > wanted ? nth(n, wanted - 1, sm, load) : ~0ull;
     __syncthreads();
     if (threadIdx.x == 0) sm.count = 0;
     __syncthreads();
@@ -1274,114 +1377,187 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
       const uint64_t c = load(i);
       if (c <= last && (c >> 32) != kNoKey) {
         const uint32_t at = atomicAdd(&sm.count, 1u);
-        if (at < kMaxCandidates) sm.pick[at] = static_cast<uint32_t>(i);  // at most `wanted`
+        if (at < kScoreCap) sm.pick[at] = static_cast<uint32_t>(i);  // at most `wanted`
       }
     }
     __syncthreads();
     have = min(static_cast<int>(sm.count), wanted);
+    if ((last >> 32) == kNoKey) last = ~0ull;
   }
   __syncthreads();
-  // distances in 64 bits, a warp to a candidate; its lanes look its rows up at once
   const T* q = x + b * ldx;
-  const int mine = have > warp ? (have - warp + kSelectWarps - 1) / kSelectWarps : 0;
-  uint32_t my_index = 0;
-  int32_t my_row = 0;
-  if (lane < mine) {
-    my_index = sm.pick[warp + kSelectWarps * lane];
-    my_row = static_cast<int32_t>(v.places.at(r.seq, my_index));
-  }
-  constexpr int kAhead = 4;  // pieces of 256 codes that are asked for at once
   const int dim = static_cast<int>(v.dim);
-  for (int c = 0; c < mine; ++c) {
-    const int64_t row = __shfl_sync(0xffffffffu, my_row, c);
-    const uint32_t i = __shfl_sync(0xffffffffu, my_index, c);
-    const uint8_t* codes = v.codes + row * v.width;
-    const uint16_t* scales = v.scales + row * v.groups;
-    const uint8_t* zeros = v.zeros ? v.zeros + row * v.groups : nullptr;
-    double sum[2] = {0.0, 0.0};
-    for (int base = 0; base < dim; base += 256 * kAhead) {
-      uint32_t packed[kAhead], bits[kAhead], zero[kAhead];
+  int kept = 0;                 // the nearest so far, in order, at the start of sm.final_*
+  int64_t next_block = 0;       // of 1024 groups
+  uint32_t at_group = 0, in_block = 0;
+  for (bool first_round = true;; first_round = false) {
+    // distances in 64 bits, a warp to a candidate; its lanes look its rows up at once
+    const int mine = have > warp ? (have - warp + kSelectWarps - 1) / kSelectWarps : 0;
+    uint32_t my_index = 0;
+    int32_t my_row = 0;
+    if (lane < mine) {
+      my_index = sm.pick[warp + kSelectWarps * lane];
+      my_row = static_cast<int32_t>(v.places.at(r.seq, my_index));
+    }
+    constexpr int kAhead = 4;  // pieces of 256 codes that are asked for at once
+    for (int c = 0; c < mine; ++c) {
+      const int64_t row = __shfl_sync(0xffffffffu, my_row, c);
+      const uint32_t i = __shfl_sync(0xffffffffu, my_index, c);
+      const uint8_t* codes = v.codes + row * v.width;
+      const uint16_t* scales = v.scales + row * v.groups;
+      const uint8_t* zeros = v.zeros ? v.zeros + row * v.groups : nullptr;
+      double sum[2] = {0.0, 0.0};
+      for (int base = 0; base < dim; base += 256 * kAhead) {
+        uint32_t packed[kAhead], bits[kAhead], zero[kAhead];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int j = base + 256 * u + 8 * lane;
-        packed[u] = 0, bits[u] = 0, zero[u] = 8;
-        if (j < dim) {
-          packed[u] = *reinterpret_cast<const uint32_t*>(codes + (j >> 1));
-          bits[u] = scales[j >> v.group_shift];
-          if (zeros) zero[u] = zeros[j >> v.group_shift] & 15u;
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int j = base + 256 * u + 8 * lane;
-        if (base + 256 * u >= dim) break;
-        const double s = v.scale_bf16
-                             ? __uint_as_float(bits[u] << 16)
-                             : __half2float(__ushort_as_half(static_cast<unsigned short>(bits[u])));
-        // 2^52 + code less 2^52 + zero: no conversion, which runs at a quarter
-        // of the rate
-        const double minus = -__hiloint2double(0x43300000, static_cast<int>(zero[u]));
-        // codes behind the last value: at the zero point, so that they count for nothing
-        uint32_t word = packed[u];
-        if (j + 8 > dim) {
-          const uint32_t keep = j < dim ? (1u << (4 * (dim - j))) - 1u : 0u;
-          word = (word & keep) | (zero[u] * 0x11111111u & ~keep);
-        }
-        double part[2] = {0.0, 0.0};
-#pragma unroll
-        for (int f = 0; f < 8; f += 2) {
-          double2 pair;
-          if constexpr (!kWide) {
-            pair = sm.query[f >> 1][j >> 3];
-          } else {
-            pair.x = j + f < dim ? static_cast<double>(load_value(q + j + f)) : 0.0;
-            pair.y = j + f + 1 < dim ? static_cast<double>(load_value(q + j + f + 1)) : 0.0;
-          }
-          const double x0 = __hiloint2double(0x43300000, (word >> (4 * f)) & 15) + minus;
-          const double x1 = __hiloint2double(0x43300000, (word >> (4 * f + 4)) & 15) + minus;
-          if constexpr (kMode == kKeyL2) {
-            const double d0 = fma(-s, x0, pair.x), d1 = fma(-s, x1, pair.y);
-            sum[0] = fma(d0, d0, sum[0]);
-            sum[1] = fma(d1, d1, sum[1]);
-          } else {
-            part[0] = fma(pair.x, x0, part[0]);
-            part[1] = fma(pair.y, x1, part[1]);
+        for (int u = 0; u < kAhead; ++u) {
+          const int j = base + 256 * u + 8 * lane;
+          packed[u] = 0, bits[u] = 0, zero[u] = 8;
+          if (j < dim) {
+            packed[u] = *reinterpret_cast<const uint32_t*>(codes + (j >> 1));
+            bits[u] = scales[j >> v.group_shift];
+            if (zeros) zero[u] = zeros[j >> v.group_shift] & 15u;
           }
         }
-        if constexpr (kMode != kKeyL2) sum[u & 1] = fma(-s, part[0] + part[1], sum[u & 1]);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int j = base + 256 * u + 8 * lane;
+          if (base + 256 * u >= dim) break;
+          const double s = v.scale_bf16
+                               ? __uint_as_float(bits[u] << 16)
+                               : __half2float(__ushort_as_half(static_cast<unsigned short>(bits[u])));
+          // 2^52 + code less 2^52 + zero: no conversion, which runs at a quarter
+          // of the rate
+          const double minus = -__hiloint2double(0x43300000, static_cast<int>(zero[u]));
+          // codes behind the last value: at the zero point, so that they count for nothing
+          uint32_t word = packed[u];
+          if (j + 8 > dim) {
+            const uint32_t keep = j < dim ? (1u << (4 * (dim - j))) - 1u : 0u;
+            word = (word & keep) | (zero[u] * 0x11111111u & ~keep);
+          }
+          double part[2] = {0.0, 0.0};
+#pragma unroll
+          for (int f = 0; f < 8; f += 2) {
+            double2 pair;
+            if constexpr (!kWide) {
+              pair = sm.query[f >> 1][j >> 3];
+            } else {
+              pair.x = j + f < dim ? static_cast<double>(load_value(q + j + f)) : 0.0;
+              pair.y = j + f + 1 < dim ? static_cast<double>(load_value(q + j + f + 1)) : 0.0;
+            }
+            const double x0 = __hiloint2double(0x43300000, (word >> (4 * f)) & 15) + minus;
+            const double x1 = __hiloint2double(0x43300000, (word >> (4 * f + 4)) & 15) + minus;
+            if constexpr (kMode == kKeyL2) {
+              const double d0 = fma(-s, x0, pair.x), d1 = fma(-s, x1, pair.y);
+              sum[0] = fma(d0, d0, sum[0]);
+              sum[1] = fma(d1, d1, sum[1]);
+            } else {
+              part[0] = fma(pair.x, x0, part[0]);
+              part[1] = fma(pair.y, x1, part[1]);
+            }
+          }
+          if constexpr (kMode != kKeyL2) sum[u & 1] = fma(-s, part[0] + part[1], sum[u & 1]);
+        }
+      }
+      double all = sum[0] + sum[1];
+#pragma unroll
+      for (int d = 16; d >= 1; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
+      if (lane == 0) {
+        const uint64_t u = static_cast<uint64_t>(__double_as_longlong(all + 0.0));
+        const bool finite = fabsf(static_cast<float>(all)) < __int_as_float(0x7f800000);
+        sm.final_key[kept + warp + kSelectWarps * c] = !finite ? ~0ull : (u >> 63) ? ~u : u | 0x8000000000000000ull;
+        sm.final_row[kept + warp + kSelectWarps * c] = i;
+        if (!finite) atomicAdd(&sm.absent, 1u);
       }
     }
-    double all = sum[0] + sum[1];
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
-    if (lane == 0) {
-      const uint64_t u = static_cast<uint64_t>(__double_as_longlong(all + 0.0));
-      const bool finite = fabsf(static_cast<float>(all)) < __int_as_float(0x7f800000);
-      sm.final_key[warp + kSelectWarps * c] = !finite ? ~0ull : (u >> 63) ? ~u : u | 0x8000000000000000ull;
-      sm.final_row[warp + kSelectWarps * c] = i;
-    }
-  }
-  __syncthreads();
-  // the place of each among all, 8 lanes to a candidate
-  int kept = 0;
-  for (int base = 0; base < have; base += kSelectThreads)
-    kept += __syncthreads_count(base + threadIdx.x < have && sm.final_key[base + threadIdx.x] != ~0ull);
-  for (int base = 0; base < have; base += kSelectThreads / 8) {
-    const int e = base + (threadIdx.x >> 3);
-    const uint64_t key = e < have ? sm.final_key[e] : 0;
-    const uint32_t index = e < have ? sm.final_row[e] : 0;
-    int rank = 0;
+    if (kMode == kKeyL2 && first_round && warp == kSelectWarps - 1) {  // |q|^2, by the warp with least to score
+      double square = 0.0;
 #pragma unroll 4
-    for (int o = threadIdx.x & 7; o < have; o += 8)
-      rank += sm.final_key[o] < key || (sm.final_key[o] == key && sm.final_row[o] < index);
+      for (int j = 2 * lane; j < dim; j += 64) {
+        double2 pair;
+        if constexpr (!kWide) {
+          pair = sm.query[(j & 7) >> 1][j >> 3];
+        } else {
+          pair.x = static_cast<double>(load_value(q + j));
+          pair.y = j + 1 < dim ? static_cast<double>(load_value(q + j + 1)) : 0.0;
+        }
+        square = fma(pair.x, pair.x, fma(pair.y, pair.y, square));
+      }
 #pragma unroll
-    for (int d = 4; d >= 1; d >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, d);
-    if ((threadIdx.x & 7) == 0 && e < have && rank < min(k, kept)) {
-      const uint64_t u = (key >> 63) ? key & 0x7fffffffffffffffull : ~key;
-      const double d = __longlong_as_double(static_cast<long long>(u));
-      neighbors[b * k + rank] = index;
-      distances[b * k + rank] = static_cast<float>(kMode == kKeyL2 ? d : -d);
+      for (int d = 16; d >= 1; d >>= 1) square += __shfl_xor_sync(0xffffffffu, square, d);
+      // from below: sums in 64 bits are off by less than 2^-30
+      if (lane == 0) sm.squared = __double2float_rd(square * (1.0 - 0x1p-30));
     }
+    __syncthreads();
+    // the place of each among all, 8 lanes to a row
+    const int all_rows = kept + have;
+    kept = min(k, all_rows - static_cast<int>(sm.absent));
+    for (int base = 0; base < all_rows; base += kSelectThreads / 8) {
+      const int e = base + (threadIdx.x >> 3);
+      const uint64_t key = e < all_rows ? sm.final_key[e] : 0;
+      const uint32_t index = e < all_rows ? sm.final_row[e] : 0;
+      int rank = 0;
+#pragma unroll 4
+      for (int o = threadIdx.x & 7; o < all_rows; o += 8)
+        rank += sm.final_key[o] < key || (sm.final_key[o] == key && sm.final_row[o] < index);
+#pragma unroll
+      for (int d = 4; d >= 1; d >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, d);
+      if ((threadIdx.x & 7) == 0 && e < all_rows && rank < kept) {
+        const uint64_t u = (key >> 63) ? key & 0x7fffffffffffffffull : ~key;
+        const double d = __longlong_as_double(static_cast<long long>(u));
+        neighbors[b * k + rank] = index;
+        distances[b * k + rank] = static_cast<float>(kMode == kKeyL2 ? d : -d);
+        sm.best_key[rank] = key;
+        sm.best_row[rank] = index;
+      }
+    }
+    __syncthreads();
+    if (first_round && last == ~0ull) break;
+    // keys up to which other rows may be as near as the k-th
+    uint32_t bound = kNoKey - 1;
+    if (kept == k) {
+      const uint64_t u = sm.best_key[k - 1];
+      const double far = __longlong_as_double(static_cast<long long>((u >> 63) ? u & 0x7fffffffffffffffull : ~u));
+      float up = __double2float_ru(far);
+      if constexpr (kMode == kKeyL2) up = __fadd_ru(__fmul_ru(up, 1.0f + 0x1p-23f), -sm.squared);
+      up += 0.0f;  // no negative zero
+      if (up < __int_as_float(0x7f800000)) bound = ordered(up);
+    }
+    if (first_round && (static_cast<uint64_t>(bound) << 32 | 0xffffffffu) <= last) break;
+    if (threadIdx.x < kept) {
+      sm.final_key[threadIdx.x] = sm.best_key[threadIdx.x];
+      sm.final_row[threadIdx.x] = sm.best_row[threadIdx.x];
+    }
+    if (threadIdx.x == 0) sm.count = sm.absent = 0;
+    __syncthreads();
+    have = 0;
+    while (have <= kScoreCap / 2) {
+      if (at_group >= in_block) {  // the groups of the next 1024 that have such keys
+        if (next_block >= groups) break;
+        if (threadIdx.x == 0) sm.groups = 0;
+        __syncthreads();
+        const int64_t g = next_block + threadIdx.x;
+        if (g < groups && minima[g] <= bound) sm.group[atomicAdd(&sm.groups, 1u)] = static_cast<int32_t>(g);
+        __syncthreads();
+        in_block = sm.groups;
+        at_group = 0;
+        next_block += kSelectThreads;
+        __syncthreads();
+        continue;
+      }
+      const uint32_t e = at_group + warp;
+      if (warp < kScoreCap / 2 / kGroupRows && e < in_block) {
+        const int64_t i = static_cast<int64_t>(sm.group[e]) * kGroupRows + lane;
+        const uint32_t key = i < n ? ordered(keys[i]) : kNoKey;
+        if (key <= bound && (static_cast<uint64_t>(key) << 32 | static_cast<uint32_t>(i)) > last)
+          sm.pick[atomicAdd(&sm.count, 1u)] = static_cast<uint32_t>(i);
+      }
+      at_group += kScoreCap / 2 / kGroupRows;
+      __syncthreads();
+      have = static_cast<int>(sm.count);
+      __syncthreads();
+    }
+    if (have == 0) break;
   }
   for (int e = kept + threadIdx.x; e < k; e += kSelectThreads) {
     neighbors[b * k + e] = -1;
@@ -1395,9 +1571,9 @@ unsigned row_grid(int64_t rows) {
 }
 
 // Shared memory of a block beside the vectors.
-int64_t mma_fixed_bytes(int split, int batch, int groups) {
+int64_t mma_fixed_bytes(int split, int batch, int groups, int mode) {
   return kMmaWarps * (kRing * kStageBytes4 + 2 * 2 * groups * kTileRows4 * 4) +
-         (split > 1 ? kMmaWarps * batch * kSumStride * 4 : 0);
+         (split > 1 ? kMmaWarps * (batch + (mode == kKeyProduct)) * kSumStride * 4 : 0);
 }
 
 // Warps that share a tile: the number with the least time of a block, in
@@ -1414,24 +1590,24 @@ int mma_split(int64_t tiles, int stages, int sms) {
   return best;
 }
 
-template <class T, int kTiles, int kParts, int kGroups, bool kZeros>
+template <class T, int kTiles, int kParts, int kGroups, bool kZeros, bool kKeyed>
 cudaError_t products(const Q4View& v, const Q4Range& r, const T* x, int batch, int64_t ldx,
                      const Q4Out& o, cudaStream_t stream) {
   constexpr int64_t kMost = 232448 - sizeof(MmaShared) - 64;
-  auto kernel = products_kernel<T, kTiles, kParts, kGroups, kZeros>;
+  auto kernel = products_kernel<T, kTiles, kParts, kGroups, kZeros, kKeyed>;
   const int sms = store_sm_count();
   MmaPlan p;
   p.tiles = (r.count + kTileRows4 - 1) / kTileRows4;
   p.stages = static_cast<int32_t>((v.dim + kStageCodes - 1) / kStageCodes);
   p.split = mma_split(p.tiles, p.stages, sms);
-  const int64_t room = (kMost - mma_fixed_bytes(p.split, batch, kGroups)) / (8 * kTiles * 512);
+  const int64_t room = (kMost - mma_fixed_bytes(p.split, batch, kGroups, o.mode)) / (8 * kTiles * 512);
   p.chunk_stages = static_cast<int32_t>(std::min<int64_t>(p.stages, room));
   while (p.split > p.chunk_stages) p.split /= 2;  // every warp has a stage of every full chunk
   p.chunks = (p.stages + p.chunk_stages - 1) / p.chunk_stages;
   const int64_t grid = std::min<int64_t>(p.tiles, sms);
   const int64_t slots = kMmaWarps / p.split;
   p.iterations = static_cast<int32_t>((p.tiles + grid * slots - 1) / (grid * slots));
-  const size_t smem = mma_fixed_bytes(p.split, batch, kGroups) + p.chunk_stages * (8 * kTiles * 512);
+  const size_t smem = mma_fixed_bytes(p.split, batch, kGroups, o.mode) + p.chunk_stages * (8 * kTiles * 512);
   static std::atomic<uint64_t> allowed{0};
   if (cudaError_t e = allow_smem(kernel, static_cast<int>(kMost), &allowed)) return e;
   store_count_launches(1);
@@ -1439,17 +1615,24 @@ cudaError_t products(const Q4View& v, const Q4Range& r, const T* x, int batch, i
                       batch, ldx, o, p);
 }
 
+template <class T, int kTiles, int kParts, bool kKeyed>
+cudaError_t products_as(const Q4View& v, const Q4Range& r, const T* x, int batch, int64_t ldx,
+                        const Q4Out& o, cudaStream_t stream) {
+  if (v.group == 32)
+    return v.zeros ? products<T, kTiles, kParts, 4, true, kKeyed>(v, r, x, batch, ldx, o, stream)
+                   : products<T, kTiles, kParts, 4, false, kKeyed>(v, r, x, batch, ldx, o, stream);
+  if (v.group == 64)
+    return v.zeros ? products<T, kTiles, kParts, 2, true, kKeyed>(v, r, x, batch, ldx, o, stream)
+                   : products<T, kTiles, kParts, 2, false, kKeyed>(v, r, x, batch, ldx, o, stream);
+  return v.zeros ? products<T, kTiles, kParts, 1, true, kKeyed>(v, r, x, batch, ldx, o, stream)
+                 : products<T, kTiles, kParts, 1, false, kKeyed>(v, r, x, batch, ldx, o, stream);
+}
+
 template <class T, int kTiles, int kParts>
 cudaError_t products_of(const Q4View& v, const Q4Range& r, const T* x, int batch, int64_t ldx,
                         const Q4Out& o, cudaStream_t stream) {
-  if (v.group == 32)
-    return v.zeros ? products<T, kTiles, kParts, 4, true>(v, r, x, batch, ldx, o, stream)
-                   : products<T, kTiles, kParts, 4, false>(v, r, x, batch, ldx, o, stream);
-  if (v.group == 64)
-    return v.zeros ? products<T, kTiles, kParts, 2, true>(v, r, x, batch, ldx, o, stream)
-                   : products<T, kTiles, kParts, 2, false>(v, r, x, batch, ldx, o, stream);
-  return v.zeros ? products<T, kTiles, kParts, 1, true>(v, r, x, batch, ldx, o, stream)
-                 : products<T, kTiles, kParts, 1, false>(v, r, x, batch, ldx, o, stream);
+  return o.mode == kStore ? products_as<T, kTiles, kParts, false>(v, r, x, batch, ldx, o, stream)
+                          : products_as<T, kTiles, kParts, true>(v, r, x, batch, ldx, o, stream);
 }
 
 // Up to kQ4SearchBatch vectors in one pass over the rows.
@@ -1529,7 +1712,7 @@ cudaError_t launch_q4_products(const Q4View& v, const Q4Range& r, const void* x,
                                cudaStream_t stream) {
   const int64_t size = dtype == KNN_DTYPE_F32 ? 4 : 2, out_size = out_dtype == KNN_DTYPE_F32 ? 4 : 2;
   for (int64_t b = 0; b < batch; b += kQ4SearchBatch) {
-    const Q4Out o = {static_cast<char*>(out) + b * ldo * out_size, out_dtype, ldo, kStore, nullptr, 0};
+    const Q4Out o = {static_cast<char*>(out) + b * ldo * out_size, out_dtype, ldo, kStore, nullptr, 0, 0.0f, 0.0f};
     if (cudaError_t e = products_any(
             v, r, static_cast<const char*>(x) + b * ldx * size, dtype,
             static_cast<int>(std::min<int64_t>(kQ4SearchBatch, batch - b)), ldx, o, stream))
@@ -1556,7 +1739,11 @@ cudaError_t launch_q4_search(const Q4View& v, const Q4Range& r, const void* x, i
     const int64_t m = std::min<int64_t>(kQ4SearchBatch, batch - b);
     const void* q = static_cast<const char*>(x) + b * ldx * size;
     if (r.count > 0) {
-      const Q4Out o = {keys, KNN_DTYPE_F32, ld, mode, minima, minima_ld(r.count)};
+      // see lowest_key; norms are held to (dim / 256 + 16) 2^-24 of them
+      const float steps = static_cast<float>(2 * v.group + v.groups + 32) * 1.001f * 0x1p-23f;
+      const Q4Out o = {keys, KNN_DTYPE_F32, ld, mode, minima, minima_ld(r.count),
+                       steps * (mode == kKeyL2 ? 2.0f : v.zeros ? 15.0f : 8.0f),
+                       static_cast<float>(v.dim / 256 + 32) * 0x1p-24f};
       if (cudaError_t e = products_any(v, r, q, dtype, static_cast<int>(m), ldx, o, stream)) return e;
     }
     cudaError_t e;

@@ -503,13 +503,15 @@ int knn_q4_products(const knn_q4_rows* q4, int64_t seq, int64_t count, const voi
 /* The k (1 .. KNN_MAX_K) nearest of the rows that knn_q4_products would
  * multiply, for each of n_queries queries: squared L2 distances to the rows'
  * 4-bit values, ascending, or inner products, descending; ties by ascending
- * index; -1 and +inf (-inf) where there are fewer.  The k + 16 best rows by
- * fp32 sums are found first and then ordered by distances summed in 64 bits,
- * which are returned rounded to fp32: the result is the exact one unless 16
- * rows or more lie within fp32's rounding (for L2, of |row|^2 - 2 q.row) at
- * the k-th place.  A row whose distance (as fp32, or for an
+ * index; -1 and +inf (-inf) where there are fewer.  Distances are summed in 64
+ * bits and returned rounded to fp32.  The k + 16 best rows by fp32 sums are
+ * looked at first, and all others that those sums' error bounds do not rule
+ * out: the result is the exact one always, and a search takes longer where
+ * fp32 cannot tell many rows apart (copies of a near row, for L2 also rows far
+ * from 0 beside their distances).  A row whose distance (as fp32, or for an
  * inner product its fp32 sums, and for L2 |row|^2 too) is no finite number is
- * no neighbour.  L2 needs the norms.  workspace: knn_q4_search_workspace bytes
+ * no neighbour.  L2 needs the norms, to (dim / 256 + 16) 2^-24 of them, as packing
+ * makes them.  workspace: knn_q4_search_workspace bytes
  * of device memory (16-byte aligned), which this call alone uses until it is
  * done. */
 int64_t knn_q4_search_workspace(int64_t count, int64_t n_queries);

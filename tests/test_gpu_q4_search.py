@@ -1,8 +1,11 @@
 """Searches of rows in 4 bits where the candidates are hard to tell: a count far
-above the sequence's length, and rows without a finite distance.
+above the sequence's length, rows without a finite distance, and rows that
+fp32 sums cannot order.
 
-Expected neighbours come from sums in 64 bits.  Distances are rounded once to
-32 bits: 2^-24 relative.
+Expected neighbours come from sums in 64 bits; where rows lie close together,
+of values with so few bits that the sums are exact there, so that ties are ties
+and go to the lowest index.  Distances are rounded once to 32 bits: 2^-24
+relative.
 """
 import math
 
@@ -169,3 +172,80 @@ def test_distances_beyond_32_bits(torch, engine):
     near, far = rows.search(q, 100)
     assert torch.equal(near[0, :50].sort().values, keep.nonzero().flatten())
     assert torch.isfinite(far[0, :50]).all() and (near[0, 50:] == -1).all() and torch.isinf(far[0, 50:]).all()
+
+
+# --------------------------------------------- rows that fp32 sums cannot order
+def close_rows(torch, engine, seed, n, small, scale, page_rows, with_norms=True):
+    """Rows that share one group of values up to 128 and differ in the other, whose
+    values are up to about `small`; every sum of their products is exact in 64 bits."""
+    rows, _ = random_rows(torch, engine, seed, n, 256, 128, False, getattr(torch, scale), page_rows)
+    order = torch.arange(n, device="cuda")
+    if page_rows:
+        order = rows.pages.table[1, order // page_rows].long() * page_rows + order % page_rows
+    codes, scales, norms = (t.view(-1, *t.shape[2:]) if page_rows else t
+                            for t in (rows.codes, rows.scales, rows.norms))
+    codes[order, :64] = codes[order[0], :64].clone()
+    scales[order, 0] = 16.0
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    scales[order, 1] = (small / 8 * (1 + torch.randint(0, 64, (n,), device="cuda", generator=g) / 64)).to(scales.dtype)
+    c = torch.stack((codes[order] & 15, codes[order] >> 4), -1).flatten(1).double() - 8
+    values = c * scales[order].double().repeat_interleave(128, 1)
+    norms[order] = values.square().sum(1).float()
+    if not with_norms:
+        rows = engine.Q4Rows(rows.codes, rows.scales, 256, 128, None, None, rows.pages)
+    return rows, values
+
+
+@pytest.mark.parametrize("n,k,batch,small,x,scale,page_rows", [
+    (4000, 8, 4, 2.0 ** -8, "float32", "float16", 0),
+    (4000, 8, 16, 2.0 ** -8, "float16", "bfloat16", 64),
+    (4000, 100, 1, 2.0 ** -5, "float16", "float16", 0),
+    (4000, 1, 3, 2.0 ** -8, "bfloat16", "float16", 48),
+    (70000, 10, 5, 2.0 ** -4, "float32", "float16", 0),
+    (70000, 256, 2, 2.0 ** -8, "bfloat16", "float16", 0),
+    (300, 256, 2, 2.0 ** -8, "float32", "float16", 0),
+])
+@pytest.mark.parametrize("metric", [0, 1])
+def test_rows_with_a_shared_offset(torch, engine, n, k, batch, small, x, scale, page_rows, metric):
+    rows, values = close_rows(torch, engine, 50 + k, n, small, scale, page_rows, with_norms=metric == 0)
+    # near the shared values, and apart from them by whole numbers
+    q = values[torch.arange(batch) * 17].clone()
+    q[:, :128] += torch.randint(-2, 3, (batch, 128), device="cuda",
+                                generator=torch.Generator(device="cuda").manual_seed(k)) * 16.0
+    q[:, 128:] = (randn(torch, 8, batch, 128).double() * small * 4).mul(2.0 ** 12).round().mul(2.0 ** -12)
+    q = q.to(getattr(torch, x))
+    got = rows.search(q, k, metric=metric, seq=1 if page_rows else None, count=n)
+    check_search(torch, got, values, torch.arange(n, device="cuda"), q, k, metric)
+
+
+@pytest.mark.parametrize("metric", [0, 1])
+def test_near_copies_of_one_row(torch, engine, metric):
+    """20,000 copies of a row, one value of some changed a little: what is exact in
+    64 bits decides, then the index."""
+    n = 20000
+    rows, _ = random_rows(torch, engine, 61, n, 256, 128, False, torch.float16)
+    rows.codes[:] = rows.codes[11].clone()
+    rows.scales[:, 0] = 8.0
+    rows.scales[:, 1] = 2.0 ** -9
+    g = torch.Generator(device="cuda").manual_seed(3)
+    changed = torch.randperm(n, device="cuda", generator=g)[:700]
+    rows.codes[changed, 100] = torch.randint(0, 256, (700,), device="cuda", generator=g, dtype=torch.uint8)
+    values = rows.read().double()
+    rows.norms[:] = values.square().sum(1).float()
+    q = values[:2].float()
+    q[:, 200:202] += torch.tensor([[0.25, -0.5], [-0.125, 1.0]], device="cuda")
+    for k in (5, 200):
+        check_search(torch, rows.search(q, k, metric=metric), values, torch.arange(n, device="cuda"), q, k, metric)
+
+
+@pytest.mark.parametrize("metric", [0, 1])
+@pytest.mark.parametrize("batch", [1, 16])
+def test_one_row_far_larger_than_the_rest(torch, engine, metric, batch):
+    """It does not make the others' order uncertain, nor lose them."""
+    n = 30000
+    rows, _ = random_rows(torch, engine, 62, n, 512, 64, True, torch.bfloat16)
+    rows.scales[[77, 20001]] *= 1e6
+    values = rows.read().double()
+    rows.norms[:] = values.square().sum(1).float()
+    q = randn(torch, 6, batch, 512)
+    check_search(torch, rows.search(q, 50, metric=metric), values, torch.arange(n, device="cuda"), q, 50, metric)
