@@ -378,9 +378,10 @@ __device__ __forceinline__ float root(float a) {
 // what |row|^2 is off by as it is held.  The sum is at most |x| |row|, and for
 // products, which need no norms, at most sum |x_j| times 15 (8 without zero
 // points) times the row's largest scale.  `size` is |row| or that scale,
-// `reach` what it is multiplied by.
+// `reach` what it is multiplied by.  2^-126 stands for what subnormal numbers
+// lose (2^13 sums of squares up to 1800 in units of 2^-150).
 __device__ __forceinline__ float lowest_key(const Q4Out& o, float y, float norm, float reach, float size) {
-  constexpr float kMost = 3.402823466e38f, kTiny = 0x1p-140f;  // kTiny: subnormal sums
+  constexpr float kMost = 3.402823466e38f, kTiny = 0x1p-126f;
   const float key = o.mode == kKeyL2 ? norm - 2.0f * y : -y;
   const float extra = o.mode == kKeyL2 ? fmaf(o.norm_slack, norm, kTiny) : kTiny;
   const float low = fmaxf(key - fminf(fmaf(reach, size, extra), kMost), -kMost);

@@ -249,3 +249,20 @@ def test_one_row_far_larger_than_the_rest(torch, engine, metric, batch):
     rows.norms[:] = values.square().sum(1).float()
     q = randn(torch, 6, batch, 512)
     check_search(torch, rows.search(q, 50, metric=metric), values, torch.arange(n, device="cuda"), q, 50, metric)
+
+
+@pytest.mark.parametrize("metric", [0, 1])
+@pytest.mark.parametrize("power", [-60, -64, -68])
+def test_rows_whose_squares_are_subnormal(torch, engine, metric, power):
+    """Squares near the smallest numbers of 32 bits: the order is that of 64 bits all
+    the same."""
+    n = 3000
+    rows, _ = random_rows(torch, engine, 63, n, 256, 128, False, torch.bfloat16)
+    j = torch.randint(0, 64, (n, 2), device="cuda", generator=torch.Generator(device="cuda").manual_seed(5))
+    rows.scales[:] = ((1 + j / 64) * 2.0 ** power).bfloat16()
+    values = rows.read().double()
+    rows.norms[:] = values.square().sum(1).float()
+    q = (values[:3] * 1.25).float()
+    near, _ = rows.search(q, 60, metric=metric)
+    want, _, _ = plain_search(torch, values, q, 60, metric)
+    assert torch.equal(near, want)
