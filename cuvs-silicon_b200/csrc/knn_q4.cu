@@ -27,15 +27,6 @@ __device__ __forceinline__ float load_value(const float* p) { return *p; }
 __device__ __forceinline__ float load_value(const __half* p) { return __half2float(*p); }
 __device__ __forceinline__ float load_value(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
-__device__ __forceinline__ float scale_of(const Q4View& v, int64_t row, int g) {
-  const uint16_t bits = v.scales[row * v.groups + g];
-  return v.scale_bf16 ? __uint_as_float(static_cast<uint32_t>(bits) << 16)
-                      : __half2float(__ushort_as_half(bits));
-}
-__device__ __forceinline__ int zero_of(const Q4View& v, int64_t row, int g) {
-  return v.zeros ? v.zeros[row * v.groups + g] & 15 : 8;
-}
-
 // The larger of two numbers, NaN where either is one.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
