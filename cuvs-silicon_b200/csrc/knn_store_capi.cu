@@ -80,6 +80,14 @@ bool is_dtype(int dtype) {
   return dtype == KNN_DTYPE_F32 || dtype == KNN_DTYPE_F16 || dtype == KNN_DTYPE_BF16;
 }
 
+// A buffer of rows in pages is one of the store's pools: what forks, compactions
+// and copies move is then all of a row.
+bool is_pool(const knn_pages& p, const void* buffer, int64_t row_bytes) {
+  for (int k = 0; k < p.n_pools; ++k)
+    if (p.pools[k] == buffer && p.row_bytes[k] == row_bytes) return true;
+  return false;
+}
+
 int check_q4(const char* what, const knn_q4_rows* q) {
   if (!q) return fail(KNN_EINVAL, "%s: null rows", what);
   if (q->dim < 1 || q->dim > KNN_Q4_MAX_DIM || (q->group != 32 && q->group != 64 && q->group != 128))
@@ -99,6 +107,13 @@ int check_q4(const char* what, const knn_q4_rows* q) {
         q->n_rows != q->pages->pages * static_cast<int64_t>(q->pages->page_rows))
       return fail(KNN_EINVAL, "%s: %lld rows do not fill the store's pages", what,
                   (long long)q->n_rows);
+    const int64_t groups = (q->dim + q->group - 1) / q->group;
+    const char* other = !is_pool(*q->pages, q->codes, knn_q4_row_bytes(q->dim)) ? "codes"
+                        : !is_pool(*q->pages, q->scales, 2 * groups)            ? "scales"
+                        : q->zeros && !is_pool(*q->pages, q->zeros, groups)     ? "zeros"
+                        : q->norms && !is_pool(*q->pages, q->norms, 4)          ? "norms"
+                                                                                : nullptr;
+    if (other) return fail(KNN_EINVAL, "%s: the %s are no pool of the store", what, other);
   }
   return KNN_OK;
 }

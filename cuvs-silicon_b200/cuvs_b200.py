@@ -577,7 +577,7 @@ class Q4Rows:
     norms   float32 [n], |row|^2, or None (only needed to search by L2)
 
     ``value = (code - zero) * scale``.  With ``pages`` the tensors are pools
-    [pages, page_rows, ...] of that store and calls name a sequence.
+    [pages, page_rows, ...] of that store, all of them, and calls name a sequence.
     """
 
     def __init__(self, codes, scales, dim: int, group: int, zeros=None, norms=None, pages=None):

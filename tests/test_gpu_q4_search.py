@@ -266,3 +266,14 @@ def test_rows_whose_squares_are_subnormal(torch, engine, metric, power):
     near, _ = rows.search(q, 60, metric=metric)
     want, _, _ = plain_search(torch, values, q, 60, metric)
     assert torch.equal(near, want)
+
+
+def test_rows_whose_norms_are_no_pool(torch, engine):
+    """A fork would leave such norms behind, and searches by L2 with them."""
+    rows, _ = random_rows(torch, engine, 71, 100, 64, 32, False, torch.float16, 16)
+    bare = engine.Pages(rows.pages.table, rows.pages.rows, rows.pages.refs, [rows.codes, rows.scales])
+    engine.Q4Rows(rows.codes, rows.scales, 64, 32, pages=bare)
+    with pytest.raises(ValueError, match="norms"):
+        engine.Q4Rows(rows.codes, rows.scales, 64, 32, norms=rows.norms, pages=bare)
+    with pytest.raises(ValueError, match="scales"):
+        engine.Q4Rows(rows.codes, rows.scales.clone(), 64, 32, norms=rows.norms, pages=rows.pages)
