@@ -49,10 +49,17 @@ int done(const char* what, cudaError_t e) {
   return fail(KNN_ECUDA, "%s: %s (%s)", what, cudaGetErrorString(e), cudaGetErrorName(e));
 }
 
+// An address that a kernel could not load a value of `size` bytes from would
+// fault the GPU.
+bool aligned(const void* p, int64_t size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
+int64_t size_of(int dtype) { return dtype == KNN_DTYPE_F32 ? 4 : 2; }
+
 int check_pages(const char* what, const knn_pages* p) {
   if (!p) return fail(KNN_EINVAL, "%s: null pages", what);
   if (!p->table || !p->rows || !p->refs || !p->status)
     return fail(KNN_EINVAL, "%s: null table, rows, refs or status", what);
+  if (!aligned(p->table, 4) || !aligned(p->rows, 4) || !aligned(p->refs, 4) || !aligned(p->status, 4))
+    return fail(KNN_EINVAL, "%s: table, rows, refs and status must be 4-byte aligned", what);
   if (p->sequences < 1 || p->sequences > KNN_PAGES_MAX_SEQUENCES || p->columns < 1 ||
       p->columns > KNN_PAGES_MAX_PAGES || p->pages < 1 || p->pages > KNN_PAGES_MAX_PAGES ||
       p->page_rows < 1 || p->pages * static_cast<int64_t>(p->page_rows) > 0x7fffffffLL)
@@ -73,6 +80,8 @@ int check_list(const char* what, int64_t n, int64_t most, const void* a, const v
     return fail(KNN_EINVAL, "%s: a list of %lld (at most %lld)", what, (long long)n,
                 (long long)most);
   if (n > 0 && (!a || !b)) return fail(KNN_EINVAL, "%s: null list", what);
+  if (n > 0 && (!aligned(a, 4) || !aligned(b, 4)))
+    return fail(KNN_EINVAL, "%s: lists must be 4-byte aligned", what);
   return KNN_OK;
 }
 
@@ -99,8 +108,8 @@ int check_q4(const char* what, const knn_q4_rows* q) {
     return fail(KNN_EINVAL, "%s: %lld rows", what, (long long)q->n_rows);
   if (q->n_rows > 0 && (!q->codes || !q->scales))
     return fail(KNN_EINVAL, "%s: null codes or scales", what);
-  if (reinterpret_cast<uintptr_t>(q->codes) % 16 != 0 || reinterpret_cast<uintptr_t>(q->scales) % 2 != 0)
-    return fail(KNN_EINVAL, "%s: codes must be 16-byte aligned, scales 2-byte", what);
+  if (!aligned(q->codes, 16) || !aligned(q->scales, 2) || !aligned(q->norms, 4))
+    return fail(KNN_EINVAL, "%s: codes must be 16-byte aligned, scales 2-byte, norms 4-byte", what);
   if (q->pages) {
     if (int st = check_pages(what, q->pages)) return st;
     if (q->pages->device != q->device ||
@@ -231,7 +240,7 @@ int knn_pages_compact(const knn_pages* p, const int32_t* sources, const int32_t*
       (keep_columns > 0 && !keep))
     return fail(KNN_EINVAL, "knn_pages_compact: keep of %lld columns, stride %lld",
                 (long long)keep_columns, (long long)keep_stride);
-  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+  if (!workspace || !aligned(workspace, 16))
     return fail(KNN_EINVAL, "knn_pages_compact: null or unaligned workspace");
   if (knn::pages_compact_words(*p, n, keep_columns) > 0x7fffffffLL)
     return fail(KNN_EUNSUPPORTED, "knn_pages_compact: %lld sequences of %lld rows in one call",
@@ -255,8 +264,8 @@ int knn_q4_pack(const knn_q4_rows* q, const void* rows, int dtype, int64_t n, in
     return fail(KNN_EINVAL, "knn_q4_pack: rows %lld .. %lld of %lld", (long long)first,
                 (long long)(first + n - 1), (long long)q->n_rows);
   if (n == 0) return KNN_OK;
-  if (!rows || (n > 1 && ld < q->dim))
-    return fail(KNN_EINVAL, "knn_q4_pack: null rows, or rows %lld apart", (long long)ld);
+  if (!rows || !aligned(rows, size_of(dtype)) || (n > 1 && ld < q->dim))
+    return fail(KNN_EINVAL, "knn_q4_pack: null or unaligned rows, or rows %lld apart", (long long)ld);
   OnDevice on(q->device);
   if (on.error()) return done("knn_q4_pack", on.error());
   return done("knn_q4_pack",
@@ -273,8 +282,8 @@ int knn_q4_append(const knn_q4_rows* q, const int32_t* seqs, const int32_t* coun
   if (total < 0 || total > q->n_rows || (total > 0 && n == 0))
     return fail(KNN_EINVAL, "knn_q4_append: %lld rows for %lld sequences", (long long)total,
                 (long long)n);
-  if (total > 0 && (!rows || (total > 1 && ld < q->dim)))
-    return fail(KNN_EINVAL, "knn_q4_append: null rows, or rows %lld apart", (long long)ld);
+  if (total > 0 && (!rows || !aligned(rows, size_of(dtype)) || (total > 1 && ld < q->dim)))
+    return fail(KNN_EINVAL, "knn_q4_append: null or unaligned rows, or rows %lld apart", (long long)ld);
   if (n == 0) return KNN_OK;
   OnDevice on(q->device);
   if (on.error()) return done("knn_q4_append", on.error());
@@ -300,8 +309,8 @@ int knn_q4_read(const knn_q4_rows* q, const int32_t* seqs, const int32_t* counts
                 (long long)(first + total - 1), (long long)q->n_rows);
   }
   if (total == 0 && !q->pages) return KNN_OK;
-  if (total > 0 && (!out || (total > 1 && ld < q->dim)))
-    return fail(KNN_EINVAL, "knn_q4_read: null output, or rows %lld apart", (long long)ld);
+  if (total > 0 && (!out || !aligned(out, 4) || (total > 1 && ld < q->dim)))
+    return fail(KNN_EINVAL, "knn_q4_read: null or unaligned output, or rows %lld apart", (long long)ld);
   OnDevice on(q->device);
   if (on.error()) return done("knn_q4_read", on.error());
   return done("knn_q4_read", knn::launch_q4_read(view_of(*q), list_of(*q, seqs, counts, n, first, total),
@@ -318,8 +327,9 @@ int knn_q4_products(const knn_q4_rows* q, int64_t seq, int64_t count, const void
     return fail(KNN_EINVAL, "knn_q4_products: types %d and %d", dtype, out_dtype);
   if (batch < 0) return fail(KNN_EINVAL, "knn_q4_products: %lld vectors", (long long)batch);
   if (batch == 0 || count == 0) return KNN_OK;
-  if (!x || !out || (batch > 1 && (ldx < q->dim || ldo < count)))
-    return fail(KNN_EINVAL, "knn_q4_products: null buffer, or rows %lld and %lld apart",
+  if (!x || !out || !aligned(x, size_of(dtype)) || !aligned(out, size_of(out_dtype)) ||
+      (batch > 1 && (ldx < q->dim || ldo < count)))
+    return fail(KNN_EINVAL, "knn_q4_products: null or unaligned buffer, or rows %lld and %lld apart",
                 (long long)ldx, (long long)ldo);
   OnDevice on(q->device);
   if (on.error()) return done("knn_q4_products", on.error());
@@ -347,9 +357,10 @@ int knn_q4_search(const knn_q4_rows* q, int64_t seq, int64_t count, const void* 
   if (n_queries == 0) return KNN_OK;
   if (metric == KNN_METRIC_L2_EXPANDED && count > 0 && !q->norms)
     return fail(KNN_EINVAL, "knn_q4_search: squared L2 distances need the rows' norms");
-  if (!queries || !neighbors || !distances || !workspace ||
-      reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || (n_queries > 1 && ld < q->dim))
-    return fail(KNN_EINVAL, "knn_q4_search: null buffer, unaligned workspace, or queries %lld apart",
+  if (!queries || !neighbors || !distances || !workspace || !aligned(queries, size_of(dtype)) ||
+      !aligned(neighbors, 8) || !aligned(distances, 4) || !aligned(workspace, 16) ||
+      (n_queries > 1 && ld < q->dim))
+    return fail(KNN_EINVAL, "knn_q4_search: null or unaligned buffer, or queries %lld apart",
                 (long long)ld);
   OnDevice on(q->device);
   if (on.error()) return done("knn_q4_search", on.error());

@@ -59,3 +59,45 @@ def test_rows_outside_their_store_are_refused(engine, name):
     lib, r = engine.lib(), ctypes.byref(q)
     assert lib.knn_q4_append(r, 4096, 4096, 1, 4096, 0, 1, 100, None) == engine.KNN_EINVAL
     assert lib.knn_q4_search(r, 0, 1, 4096, 0, 1, 100, 1, 0, 4096, 4096, 4096, None) == engine.KNN_EINVAL
+
+
+@pytest.mark.parametrize("name", ["table", "rows", "refs", "status"])
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_stores_at_odd_addresses_are_refused(engine, name, off):
+    lib = engine.lib()
+    p, q = make_store(engine)
+    assert lib.knn_pages_free(ctypes.byref(p), None, 0, None) == engine.KNN_OK
+    setattr(p, name, 4096 + off)
+    r = ctypes.byref(p)
+    assert [lib.knn_pages_free(r, None, 0, None), lib.knn_pages_copy(r, None, None, 0, None),
+            lib.knn_pages_grow(r, None, None, 0, -1, None), lib.knn_pages_fork(r, None, None, 0, None),
+            lib.knn_pages_compact(r, None, None, 0, None, 0, 0, None, None), status(engine, q)
+            ] == [engine.KNN_EINVAL] * 6
+
+
+def test_buffers_at_odd_addresses_are_refused(engine):
+    lib, (p, q) = engine.lib(), make_store(engine)
+    dense = engine.KnnQ4Rows(codes=0x10000, scales=0x20000, norms=0x40000, n_rows=512, dim=100, group=32, scale_dtype=1,
+                             device=0)
+    r, s, d = ctypes.byref(p), ctypes.byref(q), ctypes.byref(dense)
+    ok, odd, half = 4096, 4097, 4098
+    refused = [
+        lib.knn_pages_grow(r, half, ok, 1, -1, None), lib.knn_pages_grow(r, ok, half, 1, -1, None),
+        lib.knn_pages_free(r, half, 1, None), lib.knn_pages_copy(r, half, ok, 1, None),
+        lib.knn_pages_copy(r, ok, odd, 1, None), lib.knn_pages_fork(r, ok, half, 1, None),
+        lib.knn_pages_compact(r, half, ok, 1, ok, 10, 10, ok, None), lib.knn_pages_compact(r, ok, odd, 1, ok, 10, 10, ok, None),
+        lib.knn_q4_pack(d, half, 0, 1, 200, 0, None), lib.knn_q4_pack(d, odd, 1, 1, 200, 0, None),
+        lib.knn_q4_append(s, half, ok, 1, ok, 0, 1, 200, None), lib.knn_q4_append(s, ok, ok, 1, half, 0, 1, 200, None),
+        lib.knn_q4_append(s, ok, ok, 1, odd, 2, 1, 200, None),
+        lib.knn_q4_read(d, None, None, 0, 0, 1, half, 200, None), lib.knn_q4_read(s, ok, half, 1, 0, 1, ok, 200, None),
+        lib.knn_q4_products(d, -1, 10, half, 0, 1, 200, ok, 0, 10, None),
+        lib.knn_q4_products(d, -1, 10, odd, 1, 1, 200, ok, 0, 10, None),
+        lib.knn_q4_products(d, -1, 10, ok, 1, 1, 200, half, 0, 10, None),
+        lib.knn_q4_products(d, -1, 10, ok, 1, 1, 200, odd, 2, 10, None),
+        lib.knn_q4_search(d, -1, 10, half, 0, 1, 200, 5, 0, ok, ok, ok, None),
+        lib.knn_q4_search(d, -1, 10, ok, 0, 1, 200, 5, 0, ok + 4, ok, ok, None),
+        lib.knn_q4_search(d, -1, 10, ok, 0, 1, 200, 5, 0, ok, half, ok, None),
+        lib.knn_q4_search(d, -1, 10, ok, 0, 1, 200, 5, 0, ok, ok, ok + 8, None)]
+    assert refused == [engine.KNN_EINVAL] * len(refused), refused
+    dense.norms = 0x40002
+    assert lib.knn_q4_products(d, -1, 0, None, 0, 0, 0, None, 0, 0, None) == engine.KNN_EINVAL
