@@ -661,10 +661,14 @@ class Q4Rows:
     def products(self, x, seq=None, count=None, out=None, dtype=None):
         """x [batch, dim] (or one vector) times rows 0 .. count - 1: [batch,
         count] in ``dtype`` (float32 unless given).  In pages: of sequence
-        ``seq``, 0 beyond its length."""
+        ``seq``, 0 beyond its length.  Products have no gradient: an x (or out)
+        that requires one is refused, unless under torch.no_grad()."""
         torch = _torch()
         seq, count = self._range(seq, count)
         n, ldx, code = _rows_of("x", x, self.device, self.dim)
+        if (x.requires_grad or out is not None and out.requires_grad) and torch.is_grad_enabled():
+            raise ValueError("x requires a gradient, which products do not have: detach it, or call under "
+                             "torch.no_grad()")
         if count < 0 or count > self.n_rows:
             raise ValueError(f"{count} of {self.n_rows} rows")
         shape = (n, count) if x.dim() == 2 else (count,)
@@ -684,7 +688,7 @@ class Q4Rows:
 
     def search(self, queries, k: int, metric: int = METRIC_L2_EXPANDED, seq=None, count=None):
         """The k nearest rows of each query: (neighbors int64, distances
-        float32), as Index.search orders and pads them."""
+        float32, which have no gradient), as Index.search orders and pads them."""
         torch = _torch()
         seq, count = self._range(seq, count)
         n, ld, code = _rows_of("queries", queries, self.device, self.dim)

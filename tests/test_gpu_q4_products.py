@@ -121,3 +121,19 @@ def test_a_vector_gets_the_same_bits_among_others(torch, engine, x, n, dim, batc
     other = (randn(torch, 4, batch, dim) * 1e3).to(getattr(torch, x))
     other[batch // 2] = v[batch // 2]
     assert torch.equal(rows.products(other, seq=seq, count=n)[batch // 2], first[batch // 2])
+
+
+def test_a_gradient_is_refused_not_lost(torch, engine):
+    rows, _ = random_rows(torch, engine, 9, 50, 64, 32, False, torch.float16)
+    x = randn(torch, 1, 3, 64).requires_grad_()
+    for call in (lambda: rows.products(x), lambda: rows.products(x[0]),
+                 lambda: rows.products(x.detach(), out=torch.zeros(3, 50, device="cuda", requires_grad=True))):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+    want = rows.products(x.detach())
+    with torch.no_grad():
+        assert torch.equal(rows.products(x), want)
+    with torch.inference_mode():
+        assert torch.equal(rows.products(x), want)
+    # a weight that requires a gradient can be packed: its codes have none
+    assert torch.equal(engine.q4_pack(x, 32).codes, engine.q4_pack(x.detach(), 32).codes)
