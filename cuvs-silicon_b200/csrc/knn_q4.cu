@@ -390,8 +390,9 @@ __device__ __forceinline__ void put(const Q4Out& o, int64_t b, int64_t i, float 
 // The products run on the warp's own matrix instructions (mma.sync, fp16 in,
 // fp32 sums): a row's partial sums have to be scaled after every 32 to 128
 // values, which in registers is one multiply-add to a sum, while sums in
-// tensor memory would have to be read out and scaled that often, and scales
-// multiplied into the weights would no longer be exact in 16 bits.  A code
+// tensor memory would have to be read out and scaled that often (a form that
+// was not built, so not measured), and scales multiplied into the weights
+// would no longer be exact in 16 bits.  A code
 // less its zero point is a whole number of at most 5 bits, so every product
 // in the matrix unit is exact, and the rounding is that of fp32 sums.
 //
@@ -415,7 +416,9 @@ __device__ __forceinline__ void put(const Q4Out& o, int64_t b, int64_t i, float 
 // barrier between warps); the ring also hands the codes of a group to the
 // lanes that the matrix instruction wants them in.  The order of the values
 // within a group is free as long as codes and vector agree, so codes are
-// unpacked where they lie:
+// unpacked where they lie, by the published way of placing whole numbers in
+// the fraction of fp16's 1024 (Kim, Henry, Fahim and Hassan Awadalla, "Who says
+// elephants can't run", 2022):
 //   word of 8 codes, & 0x000f000f | 0x64006400 = (1024 + c0, 1024 + c4) in
 //   fp16, & 0x00f000f0 likewise (1024 + 16 c1, 1024 + 16 c5), and both again
 //   8 bits further; one fp16 instruction takes off 1024 + zero (and the 16).
@@ -424,13 +427,18 @@ __device__ __forceinline__ void put(const Q4Out& o, int64_t b, int64_t i, float 
 // up through shared memory, in order.
 //
 // Measured (B200; rows of 1024 values in groups of 64, a million of them):
-// 1 to 8 fp16 vectors 117 us, 16 of them 156 us (0.61 of the copy bandwidth
-// that the 608 MB would allow), 16 fp32 ones 244 us; 1 fp32 vector x 10,000
-// rows 9 us, the call included.  Copying alone, without the products, takes 92 us.  What bounds it
-// is issuing: 350 instructions for 32 rows x 128 codes, of which unpacking is
-// 144, the matrix unit 32 (busy 40% of the time), scaling 32; 12 warps take as
-// long as 16.  Unpacking by ANDs alone, with the zero points taken off by one
-// more matrix product a group, has 64 fewer but was 6% slower.
+// 1 to 8 fp16 vectors 112 us, 16 of them 146 us (0.64 of the copy bandwidth
+// that the 608 MB would allow), 16 fp32 ones 218 us; 1 fp32 vector x 10,000
+// rows 9 us, the call included; bf16 scales with bf16 or fp32 vectors 4 to 7% more
+// than fp16 ones.  Copying alone, without the products, takes 92 us.  No unit is
+// busy all the time: with 4 warps a scheduler (128 registers a thread, one
+// block a multiprocessor) an instruction is issued in 56% of the cycles, and
+// warps mostly wait for a math pipe (1.4 cycles an instruction) or for the fixed
+// latency of the instruction before (1.3); the matrix unit is busy 41% of the
+// time, the integer pipe 37%, DRAM 43%.  32 rows x 128 codes are 350
+// instructions, of which unpacking is 144, the matrix unit's 32, scaling 32; 12
+// warps take as long as 16.  Unpacking by ANDs alone, with the zero points taken
+// off by one more matrix product a group, has 64 fewer but was 6% slower.
 constexpr int kMmaWarps = 16;
 constexpr int kMmaThreads = 32 * kMmaWarps;
 constexpr int kTileRows4 = 32;    // rows of a tile
@@ -1268,8 +1276,8 @@ __device__ void sort_candidates(SelectSmem& sm, int n) {
 // c rows lie at or below tau, so only keys <= tau are looked at, and they are
 // in the groups whose minimum is <= tau: c groups, unless keys are equal.
 //
-// A latency: one CTA goes through it query by query.  Measured: 11 us for the
-// 10 nearest of 125,000 rows of 1024 values, 30 us for the 100 nearest of a
+// A latency: one CTA goes through it for each query.  Measured: 12 us for the
+// 10 nearest of 125,000 rows of 1024 values, 31 us for the 100 nearest of a
 // million for each of 16 queries, about half of it the scoring.
 template <class T, int kMode, bool kWide>
 __global__ void __launch_bounds__(kSelectThreads) select_kernel(
