@@ -1097,7 +1097,7 @@ struct SelectSmem {
   uint64_t best_key[KNN_MAX_K];
   uint32_t best_row[KNN_MAX_K];
   float squared;    // |q|^2 from below
-  uint32_t absent;  // scored rows that are at no finite distance
+  uint32_t fresh;   // rows just scored that are among the nearest so far
   uint32_t hist[kBins];
   uint32_t part[32];
   int32_t group[kGroupCap];
@@ -1269,8 +1269,8 @@ __device__ void sort_candidates(SelectSmem& sm, int n) {
 // 1024 at a time, while the k-th distance comes down: the result is the exact
 // one always, and such a search takes longer the more rows there are that
 // fp32 cannot tell apart (a million rows of 1024 values, one query, k = 10: 0.15
-// ms, with 1000 copies of the nearest 0.32, with 10,000 of them 3.8, with 100,000
-// 18).
+// ms, with 1000 copies of the nearest 0.25, with 10,000 of them 3.0, most of it
+// the pass over all keys, with 100,000 10).
 //
 // Candidates: with c wanted and tau the c-th smallest of the groups' minima,
 // c rows lie at or below tau, so only keys <= tau are looked at, and they are
@@ -1300,7 +1300,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
     double2& pair = sm.query[(j & 7) >> 1][j >> 3];
     (j & 1 ? pair.y : pair.x) = value;
   }
-  if (threadIdx.x == 0) sm.absent = 0;
+  if (threadIdx.x == 0) sm.fresh = 0;
   __syncthreads();
   if (groups > wanted) tau = min(minima_bound(minima, groups, wanted, sm), kNoKey - 1);
   __syncthreads();
@@ -1462,12 +1462,15 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
       double all = sum[0] + sum[1];
 #pragma unroll
       for (int d = 16; d >= 1; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
-      if (lane == 0) {
+      if (lane == 0 && fabsf(static_cast<float>(all)) < __int_as_float(0x7f800000)) {
         const uint64_t u = static_cast<uint64_t>(__double_as_longlong(all + 0.0));
-        const bool finite = fabsf(static_cast<float>(all)) < __int_as_float(0x7f800000);
-        sm.final_key[kept + warp + kSelectWarps * c] = !finite ? ~0ull : (u >> 63) ? ~u : u | 0x8000000000000000ull;
-        sm.final_row[kept + warp + kSelectWarps * c] = i;
-        if (!finite) atomicAdd(&sm.absent, 1u);
+        const uint64_t key = (u >> 63) ? ~u : u | 0x8000000000000000ull;
+        // of a later round only what comes before the k-th so far
+        if (kept < k || key < sm.best_key[k - 1] || (key == sm.best_key[k - 1] && i < sm.best_row[k - 1])) {
+          const uint32_t at = kept + atomicAdd(&sm.fresh, 1u);
+          sm.final_key[at] = key;
+          sm.final_row[at] = i;
+        }
       }
     }
     if (kMode == kKeyL2 && first_round && warp == kSelectWarps - 1) {  // |q|^2, by the warp with least to score
@@ -1490,9 +1493,9 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
     }
     __syncthreads();
     // the place of each among all, 8 lanes to a row
-    const int all_rows = kept + have;
-    kept = min(k, all_rows - static_cast<int>(sm.absent));
-    for (int base = 0; base < all_rows; base += kSelectThreads / 8) {
+    const int fresh = static_cast<int>(sm.fresh), all_rows = kept + fresh;
+    kept = min(k, all_rows);
+    for (int base = 0; fresh > 0 && base < all_rows; base += kSelectThreads / 8) {
       const int e = base + (threadIdx.x >> 3);
       const uint64_t key = e < all_rows ? sm.final_key[e] : 0;
       const uint32_t index = e < all_rows ? sm.final_row[e] : 0;
@@ -1528,7 +1531,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(
       sm.final_key[threadIdx.x] = sm.best_key[threadIdx.x];
       sm.final_row[threadIdx.x] = sm.best_row[threadIdx.x];
     }
-    if (threadIdx.x == 0) sm.count = sm.absent = 0;
+    if (threadIdx.x == 0) sm.count = sm.fresh = 0;
     __syncthreads();
     have = 0;
     while (have <= kScoreCap / 2) {

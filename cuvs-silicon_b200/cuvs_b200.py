@@ -574,7 +574,8 @@ class Q4Rows:
     codes   uint8 [n, 16 * ceil(dim / 32)], two codes a byte, the first low
     scales  float16 or bfloat16 [n, ceil(dim / group)], group 32, 64 or 128
     zeros   uint8 like scales, or None: 8 throughout
-    norms   float32 [n], |row|^2, or None (only needed to search by L2)
+    norms   float32 [n], |row|^2 to (dim / 256 + 16) 2^-24 of it, as packing makes
+            them, or None (only needed to search by L2)
 
     ``value = (code - zero) * scale``.  With ``pages`` the tensors are pools
     [pages, page_rows, ...] of that store, all of them, and calls name a sequence.

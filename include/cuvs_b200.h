@@ -384,7 +384,9 @@ int knn_selftest_bounded_wait(int device, int64_t limit_us);
  * pools share the page numbers.  refs[p] counts the table entries that hold
  * page p; a page without any is free.  Table entries at and beyond
  * ceil(rows[s] / page_rows) are -1.  A new store has table = -1 and rows =
- * refs = 0 throughout. */
+ * refs = 0 throughout.  An entry within a sequence's length that is no page's
+ * number is read as rows that are missing (see knn_q4_products); copies of such
+ * rows that a fork or compaction makes hold anything. */
 typedef struct knn_pages {
   int32_t* table;      /* [sequences][columns] */
   int32_t* rows;       /* [sequences]: lengths */
