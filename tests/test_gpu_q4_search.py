@@ -268,6 +268,50 @@ def test_rows_whose_squares_are_subnormal(torch, engine, metric, power):
     assert torch.equal(near, want)
 
 
+@pytest.mark.parametrize("metric", [0, 1])
+@pytest.mark.parametrize("x", ["float32", "float16"])
+def test_near_copies_of_wide_rows(torch, engine, metric, x):
+    """Rows wider than a query that is kept on chip, more queries than one pass takes."""
+    n, dim = 900, 8300
+    rows, _ = random_rows(torch, engine, 64, n, dim, 128, False, torch.float16)
+    rows.codes[:] = rows.codes[0].clone()
+    rows.scales[:] = 2.0 ** -9
+    rows.scales[:, 0] = 16.0
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rows.codes[:, 4100:4140] = torch.randint(0, 256, (n, 40), device="cuda", generator=g, dtype=torch.uint8)
+    rows.codes[300:500] = rows.codes[7].clone()
+    values = rows.read().double()
+    rows.norms[:] = values.square().sum(1).float()
+    q = values[torch.arange(18) * 50].to(getattr(torch, x))
+    q[:, 8200:8290] += (torch.randint(-9, 10, (18, 90), device="cuda", generator=g) * 2.0 ** -9).to(q.dtype)
+    for k in (1, 30):
+        check_search(torch, rows.search(q, k, metric=metric), values, torch.arange(n, device="cuda"), q, k, metric)
+
+
+def test_easy_and_hard_queries_of_one_graph(torch, engine):
+    """A captured search whose queries need more rows scored in one replay than in another."""
+    n = 5000
+    rows, values = close_rows(torch, engine, 65, n, 2.0 ** -8, "float16", 64)
+    index = torch.arange(n, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(5)
+
+    def queries(hard):
+        q = values[torch.arange(3) * 100].clone()
+        q[:, 128:] = torch.randint(-9, 10, (3, 128), device="cuda", generator=g) * 2.0 ** (-9 if hard else 7)
+        return q.float()
+
+    q = queries(True)
+    rows.search(q, 20, seq=1, count=n)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = rows.search(q, 20, seq=1, count=n)
+    for hard in (True, False, True, False):
+        q.copy_(queries(hard))
+        graph.replay()
+        check_search(torch, got, values, index, q, 20, 0)
+
+
 def test_rows_whose_norms_are_no_pool(torch, engine):
     """A fork would leave such norms behind, and searches by L2 with them."""
     rows, _ = random_rows(torch, engine, 71, 100, 64, 32, False, torch.float16, 16)
